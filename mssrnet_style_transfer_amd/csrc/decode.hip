@@ -325,7 +325,8 @@ __device__ __forceinline__ float dot16_packed(const typename Row16<T>::V& a, con
     }
 }
 
-// acc += w * row, two elements per instruction (v_pk_fma_f32 on adjacent accumulator registers)
+// acc += w * row, written on adjacent accumulator pairs (compiled to one v_fma_f32 an element: the build turns packed
+// fp32 instructions off)
 template <typename T>
 __device__ __forceinline__ void axpy16(float (&acc)[Row16<T>::E], float w, const typename Row16<T>::V& x) {
     typedef float f2 __attribute__((ext_vector_type(2)));
