@@ -627,6 +627,43 @@ typedef struct {
 int mssr_decstack_fwd(const mssr_decstack_plan* plan, void* stream);
 int mssr_decstack_bwd(const mssr_decstack_plan* plan, void* stream);
 
+/* ------------------------------------------------- 4-bit key/value cache and attention over it --
+ * A decoder's cached keys and values (state["cache"] of onmt/decoders/transformer.py:268-287, the layer_cache of
+ * onmt/modules/multi_headed_attn.py:131-160) held in 4 bits: codes with an fp16 scale and zero for every 32 features of a
+ * token and head, value = zero + scale * code; csrc/kv4.hpp states the numbers and the layout.  5 bits a feature against
+ * 16 or 32.  `data` is mssr_kv4_bytes() bytes of the caller, 16-byte aligned, initialised or not: only tokens that a call
+ * writes change, and what lies past a sentence's length is never used.  dh: a multiple of 8 up to 128.
+ *
+ * Index tables (start, counts, lengths) are device arrays of B integers, 32-bit unless the matching flag says 64; a NULL
+ * start / lengths means the scalar beside it for every sentence, NULL counts means T.  Their values are not checked on the
+ * host: positions outside [0, capacity) are not written and read as zero, lengths are clamped to [0, capacity].
+ * Strides are in elements, the features of a row are contiguous, no further alignment is needed. */
+typedef struct {
+    void* data;
+    int64_t B, capacity;          /* sentences; tokens a sentence may hold */
+    int H, dh;                    /* key/value heads, features of a head */
+} mssr_kv4_cache;
+int64_t mssr_kv4_bytes(int64_t B, int H, int64_t capacity, int dh);     /* < 0: not a valid shape */
+
+/* Quantises tokens t < min(T, counts[b]) of k, v (element (b, h, t, c) at b*bs + h*hs + t*ts + c) to the positions
+ * start[b] + t.  index_bits: 1 = start is int64, 2 = counts is int64. */
+int mssr_kv4_write(const mssr_kv4_cache* cache, const void* k, int64_t k_bs, int64_t k_hs, int64_t k_ts, const void* v,
+                   int64_t v_bs, int64_t v_hs, int64_t v_ts, int64_t T, const void* start, int64_t start0,
+                   const void* counts, int index_bits, int dtype, void* stream);
+/* The values that positions start[b] + t, t < min(T, counts[b]) stand for, rounded once to dtype; zero for the other t < T. */
+int mssr_kv4_read(const mssr_kv4_cache* cache, void* k, int64_t k_bs, int64_t k_hs, int64_t k_ts, void* v, int64_t v_bs,
+                  int64_t v_hs, int64_t v_ts, int64_t T, const void* start, int64_t start0, const void* counts,
+                  int index_bits, int dtype, void* stream);
+/* out = softmax(scale * q k^T) v of Tq query rows over the first lengths[b] cached tokens (causal: row i over the first
+ * lengths[b] - Tq + 1 + i); a row that sees no token gives zeros.  H query heads, a multiple of the cache's: head h reads
+ * key/value head h / (H / cache->H).  `longest`: an upper bound of the lengths if the caller knows one (0: the capacity);
+ * it only shapes the launch.  scratch: mssr_kv4_attention_scratch() bytes, free again when the call's work is done. */
+int64_t mssr_kv4_attention_scratch(const mssr_kv4_cache* cache, int64_t Tq, int H, int64_t longest, int dtype);
+int mssr_kv4_attention(const mssr_kv4_cache* cache, const void* q, int64_t q_bs, int64_t q_hs, int64_t q_ts, void* out,
+                       int64_t o_bs, int64_t o_hs, int64_t o_ts, int H, int64_t Tq, const void* lengths, int64_t length0,
+                       int lengths_are_64, int64_t longest, float scale, int causal, void* scratch, int64_t scratch_bytes,
+                       int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

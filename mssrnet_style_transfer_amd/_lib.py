@@ -95,6 +95,11 @@ class AttnDesc(Structure):
                 ("p_drop", c_float), ("seed", c_uint64), ("dtype", c_int), ("drop_b0", c_int)]
 
 
+class Kv4Cache(Structure):
+    """mssr_kv4_cache (include/mssr_hip.h)."""
+    _fields_ = [("data", c_void_p), ("B", c_int64), ("capacity", c_int64), ("H", c_int), ("dh", c_int)]
+
+
 class PackJob(Structure):
     """mssr_pack_job (include/mssr_hip.h)."""
     _fields_ = [("src", c_void_p), ("rows", c_int), ("cols", c_int), ("dst", c_void_p), ("dst_ld", c_int64),
@@ -168,6 +173,12 @@ SIGNATURES = {
     "mssr_decode_graphs": ([], c_int),
     "mssr_decode_graphs_recorded": ([], ctypes.c_long),
     "mssr_decode_graphs_enable": ([_I], c_int),
+    "mssr_kv4_bytes": ([_L, _I, _L, _I], c_int64),
+    "mssr_kv4_write": ([POINTER(Kv4Cache), _P, _L, _L, _L, _P, _L, _L, _L, _L, _P, _L, _P, _I, _I, _P], c_int),
+    "mssr_kv4_read": ([POINTER(Kv4Cache), _P, _L, _L, _L, _P, _L, _L, _L, _L, _P, _L, _P, _I, _I, _P], c_int),
+    "mssr_kv4_attention_scratch": ([POINTER(Kv4Cache), _L, _I, _L, _I], c_int64),
+    "mssr_kv4_attention": ([POINTER(Kv4Cache), _P, _L, _L, _L, _P, _L, _L, _L, _I, _L, _P, _L, _I, _L, _F, _I, _P, _L, _I, _P],
+                           c_int),
     "mssr_debug_stamps": ([_P], None),
     "mssr_ctx_kv_grad": ([_P, _P, _L, _P, _L, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P], c_int),
 }
