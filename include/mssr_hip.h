@@ -664,6 +664,41 @@ int mssr_kv4_attention(const mssr_kv4_cache* cache, const void* q, int64_t q_bs,
                        int lengths_are_64, int64_t longest, float scale, int causal, void* scratch, int64_t scratch_bytes,
                        int dtype, void* stream);
 
+/* --------------------------------------------------------- control of the next token's logits --
+ * What a decoding step does to its logits before it picks (the search of onmt/translate/greedy_search.py:135-165 and the
+ * n-gram rule of onmt/translate/decode_strategy.py): penalties for tokens of the history, a bias, a grammar's mask, no
+ * repeated n-gram; the arithmetic is stated in csrc/token_control.hip.  Writes the new logits (out), the pick (ids: the
+ * largest, lowest index on ties, NaN above everything, `empty` where nothing is left), or both; out may be logits itself.
+ * Index arrays hold 32-bit integers, or 64-bit ones where their bit of index_bits is set.  Nothing in them is checked on the
+ * host: history entries outside [0, V) are passed over, lengths are clamped to [0, T], a state below 0 leaves its row free,
+ * one beyond the table allows nothing. */
+typedef struct {
+    const void* logits;           /* [B, V] of dtype, row stride ld */
+    void* out;                    /* [B, V] of dtype, row stride ldo, or NULL */
+    int64_t B, V, ld, ldo;
+    const void* history;          /* token t of row b at b*h_bs + t*h_ts, t < T; NULL: no history */
+    int64_t h_bs, h_ts, T;
+    const void* lengths;          /* [B] tokens of a row's history, or NULL: T */
+    const void* prompt_lengths;   /* [B] where counting (frequency, presence) begins, or NULL: 0 */
+    const float *repetition, *frequency, *presence;      /* [B], or NULL: the scalars */
+    float repetition0, frequency0, presence0;
+    int ngram;                    /* n >= 1: no n-gram twice; 0: off */
+    const float* bias;            /* [V] (bias_bs = 0) or rows bias_bs apart, or NULL */
+    int64_t bias_bs;
+    const void* allowed;          /* bit v % 32 of 32-bit word v / 32 of a state's row, rows of (V + 31) / 32 words, or NULL */
+    int64_t states;
+    const void* state;            /* [B] row of `allowed` for each row (state_mode 2) */
+    int state_mode;               /* 0: row 0 for all, 1: row b, 2: state[b] */
+    void* ids;                    /* [B] picks, or NULL */
+    int64_t empty;
+    int index_bits;               /* 64-bit: 1 history, 2 lengths, 4 prompt_lengths, 8 state, 16 ids */
+    int dtype;
+    void* scratch;                /* mssr_token_control_scratch() bytes where ids is given */
+    int64_t scratch_bytes;
+} mssr_token_control_desc;
+int64_t mssr_token_control_scratch(int64_t B, int64_t V);
+int mssr_token_control(const mssr_token_control_desc* desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

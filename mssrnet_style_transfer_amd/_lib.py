@@ -100,6 +100,17 @@ class Kv4Cache(Structure):
     _fields_ = [("data", c_void_p), ("B", c_int64), ("capacity", c_int64), ("H", c_int), ("dh", c_int)]
 
 
+class TokenControlDesc(Structure):
+    """mssr_token_control_desc (include/mssr_hip.h)."""
+    _fields_ = [("logits", c_void_p), ("out", c_void_p), ("B", c_int64), ("V", c_int64), ("ld", c_int64), ("ldo", c_int64),
+                ("history", c_void_p), ("h_bs", c_int64), ("h_ts", c_int64), ("T", c_int64), ("lengths", c_void_p),
+                ("prompt_lengths", c_void_p), ("repetition", c_void_p), ("frequency", c_void_p), ("presence", c_void_p),
+                ("repetition0", c_float), ("frequency0", c_float), ("presence0", c_float), ("ngram", c_int),
+                ("bias", c_void_p), ("bias_bs", c_int64), ("allowed", c_void_p), ("states", c_int64), ("state", c_void_p),
+                ("state_mode", c_int), ("ids", c_void_p), ("empty", c_int64), ("index_bits", c_int), ("dtype", c_int),
+                ("scratch", c_void_p), ("scratch_bytes", c_int64)]
+
+
 class PackJob(Structure):
     """mssr_pack_job (include/mssr_hip.h)."""
     _fields_ = [("src", c_void_p), ("rows", c_int), ("cols", c_int), ("dst", c_void_p), ("dst_ld", c_int64),
@@ -179,6 +190,8 @@ SIGNATURES = {
     "mssr_kv4_attention_scratch": ([POINTER(Kv4Cache), _L, _I, _L, _I], c_int64),
     "mssr_kv4_attention": ([POINTER(Kv4Cache), _P, _L, _L, _L, _P, _L, _L, _L, _I, _L, _P, _L, _I, _L, _F, _I, _P, _L, _I, _P],
                            c_int),
+    "mssr_token_control_scratch": ([_L, _L], c_int64),
+    "mssr_token_control": ([POINTER(TokenControlDesc), _P], c_int),
     "mssr_debug_stamps": ([_P], None),
     "mssr_ctx_kv_grad": ([_P, _P, _L, _P, _L, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P], c_int),
 }

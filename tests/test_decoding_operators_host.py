@@ -1,0 +1,125 @@
+"""Refusals of the decoding operators' C entry points (include/mssr_hip.h): every bad shape is an error code before
+anything is launched, so these run without a GPU; and the host-side helpers."""
+import ctypes
+
+import pytest
+import torch
+
+from mssrnet_style_transfer_amd import _lib as L
+from mssrnet_style_transfer_amd.token_control import TokenControl, pack_allowed
+
+FAKE = 1 << 20          # an address that no call here may reach
+
+
+def cache(B=2, H=2, capacity=100, dh=64, data=FAKE):
+    return L.Kv4Cache(data, B, capacity, H, dh)
+
+
+def test_cache_sizes():
+    lib = L.load()
+    assert lib.mssr_kv4_bytes(1, 1, 1, 8) == 2560
+    assert lib.mssr_kv4_bytes(3, 2, 65, 64) == 3 * 2 * 2 * 2 * 2560
+    assert lib.mssr_kv4_bytes(2, 8, 1 << 24, 128) == 2 * 8 * (1 << 18) * 4 * 2560
+    for B, H, cap, dh in ((0, 1, 1, 64), (1, 0, 1, 64), (1, 1, 0, 64), (1, 1, 1, 0), (1, 1, 1, 60), (1, 1, 1, 136),
+                          (-1, 1, 1, 64), (1, 1, -1, 64), (1 << 40, 8, 1 << 40, 128), (1, 1, 1 << 62, 64)):
+        assert lib.mssr_kv4_bytes(B, H, cap, dh) == -1, (B, H, cap, dh)
+
+
+@pytest.mark.parametrize("fn", ["mssr_kv4_write", "mssr_kv4_read"])
+def test_cache_refusals(fn):
+    lib = L.load()
+
+    def call(c, k=FAKE, v=FAKE, T=3, start=None, start0=0, counts=None, bits=0, dtype=L.F32):
+        return getattr(lib, fn)(ctypes.byref(c), k, 0, 0, 64, v, 0, 0, 64, T, start, start0, counts, bits, dtype, None)
+
+    for c in (cache(data=None), cache(dh=60), cache(dh=0), cache(dh=256), cache(B=0), cache(H=0), cache(capacity=0),
+              cache(data=FAKE + 8)):
+        assert call(c) == 1
+    for kw in (dict(k=None), dict(v=None), dict(T=-1), dict(dtype=2), dict(dtype=-1), dict(T=101), dict(start0=98),
+               dict(start0=-1), dict(bits=4), dict(start0=1 << 62), dict(T=1 << 62)):
+        assert call(cache(), **kw) == 1, kw
+    # more heads x blocks than one grid has room for
+    assert call(cache(B=1 << 24, H=8, capacity=1 << 20), T=1 << 19) == 1
+    assert lib.mssr_last_error()
+    assert call(cache(), k=None, v=None, T=0) == 0                          # no tokens: nothing to do
+
+
+def test_attention_refusals():
+    lib = L.load()
+
+    def call(c, q=FAKE, out=FAKE, H=2, Tq=1, lengths=None, n=10, longest=0, scratch=None, nbytes=0, dtype=L.F32):
+        return lib.mssr_kv4_attention(ctypes.byref(c), q, 0, 0, 64, out, 0, 0, 64, H, Tq, lengths, n, 0, longest, 1.0, 0,
+                                      scratch, nbytes, dtype, None)
+
+    for c in (cache(data=None), cache(dh=60), cache(dh=160), cache(B=0), cache(H=0), cache(capacity=0), cache(data=FAKE + 4)):
+        assert call(c) == 1
+    for kw in (dict(q=None), dict(out=None), dict(H=3), dict(H=1), dict(H=0), dict(Tq=-1), dict(dtype=2), dict(n=101),
+               dict(n=-1), dict(Tq=1 << 40), dict(Tq=(1 << 31) - 1)):
+        assert call(cache(), **kw) == 1, kw
+    # a long cache of few heads is split, which takes scratch
+    c = cache(B=1, capacity=100000)
+    need = lib.mssr_kv4_attention_scratch(ctypes.byref(c), 1, 2, 0, L.F32)
+    assert need > 0 and call(c, n=100000) == 1 and call(c, n=100000, scratch=FAKE, nbytes=need - 1) == 1
+    assert lib.mssr_kv4_attention_scratch(ctypes.byref(cache(capacity=64)), 1, 2, 0, L.F32) == 0
+    for kw in (dict(Tq=0), dict(H=3), dict(dtype=5), dict(Tq=1 << 40)):
+        a = {**dict(Tq=1, H=2, dtype=0), **kw}
+        assert lib.mssr_kv4_attention_scratch(ctypes.byref(c), a["Tq"], a["H"], 0, a["dtype"]) == -1
+    assert call(cache(), q=None, out=None, Tq=0) == 0
+
+
+def control(**kw):
+    d = L.TokenControlDesc()
+    d.logits, d.out, d.B, d.V, d.ld, d.ldo, d.repetition0 = FAKE, FAKE, 2, 50, 50, 50, 1.0
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return L.load().mssr_token_control(ctypes.byref(d), None)
+
+
+def test_token_control_refusals():
+    for kw in (dict(logits=None), dict(out=None), dict(V=0), dict(V=1 << 31), dict(ld=49), dict(ldo=49), dict(B=-1),
+               dict(dtype=2), dict(T=-1), dict(T=1 << 30), dict(ngram=-1), dict(ngram=65),
+               dict(allowed=FAKE, states=0), dict(allowed=FAKE, states=1, state_mode=1),
+               dict(allowed=FAKE, states=9, state_mode=2), dict(allowed=FAKE, states=9, state_mode=3),
+               dict(B=1 << 40), dict(ids=FAKE, V=100000, ld=100000, ldo=100000)):
+        assert control(**kw) == 1, kw
+    assert L.load().mssr_token_control(None, None) == 1
+    assert control(B=0, logits=None) == 0
+    lib = L.load()
+    assert lib.mssr_token_control_scratch(0, 5) == -1 and lib.mssr_token_control_scratch(1, 0) == -1
+    assert lib.mssr_token_control_scratch(1, 20) == 0 and lib.mssr_token_control_scratch(1, 100000) > 0
+
+
+def test_pack_allowed():
+    g = torch.Generator().manual_seed(3)
+    for S, V in ((1, 1), (2, 32), (3, 33), (2, 95)):
+        a = torch.rand(S, V, generator=g) < 0.5
+        w = pack_allowed(a)
+        assert w.dtype == torch.int32 and w.shape == (S, (V + 31) // 32)
+        bits = torch.tensor([[(int(w[s, v // 32]) >> (v % 32)) & 1 for v in range(V)] for s in range(S)], dtype=torch.bool)
+        assert torch.equal(bits, a)
+        assert V % 32 == 0 or all((int(x) & 0xffffffff) >> (V % 32) == 0 for x in w[:, -1])
+    with pytest.raises(ValueError):
+        pack_allowed(torch.ones(3, 4))
+
+
+def test_rows_of_a_control():
+    index = torch.tensor([2, 0])
+    c = TokenControl(repetition=torch.arange(3.0), frequency=0.5, bias=torch.arange(6.0).view(3, 2),
+                     allowed=torch.arange(4).view(4, 1).int(), state=torch.tensor([5, 6, 7]))
+    r = c.rows(index, 3)
+    assert r.repetition.tolist() == [2, 0] and r.frequency == 0.5 and r.bias.tolist() == [[4, 5], [0, 1]]
+    assert r.state.tolist() == [7, 5] and r.allowed is c.allowed
+    each = TokenControl(bias=torch.zeros(2), allowed=torch.arange(3).view(3, 1).int()).rows(index, 3)
+    assert each.allowed.view(-1).tolist() == [2, 0] and each.bias.shape == (2,)
+    one = TokenControl(allowed=torch.arange(1).view(1, 1).int()).rows(index, 3)
+    assert one.allowed.shape == (1, 1)
+
+
+def test_cpu_tensors_are_refused():
+    from mssrnet_style_transfer_amd import kv_cache, token_control
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        kv_cache.KVCache4(1, 1, 64, 4, device="cpu")
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        token_control.pick_token(torch.zeros(2, 5))
+    with pytest.raises(ValueError):
+        kv_cache.KVCache4(1, 1, 60, 4, device="cpu")
