@@ -43,6 +43,7 @@ __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
 // The group's codes of this lane's 8 features (one byte each, features 0-3 in c0, 4-7 in c1) and its (s, z) word.
 // `live`: the lane holds features (a head's last group may have fewer than 32).  All four lanes of a group call it.
 __device__ __forceinline__ void kv4_quantise(float (&x)[8], bool live, uint32_t& c0, uint32_t& c1, uint32_t& meta) {
+#pragma clang fp contract(off)
     float lo = INFINITY, hi = -INFINITY;
     uint32_t bad = 0;
 #pragma unroll
@@ -59,8 +60,12 @@ __device__ __forceinline__ void kv4_quantise(float (&x)[8], bool live, uint32_t&
     lo = fminf(lo, dpp_mov<0x4E>(lo));
     hi = fmaxf(hi, dpp_mov<0x4E>(hi));
     bad |= dpp_u32<0x4E>(bad);
-    f16 s = (f16)((hi - lo) * (1.0f / 15.0f));       // rounding to nearest even: the scale a code is multiplied by
-    f16 z = (f16)lo;
+    float step = (hi - lo) * (1.0f / 15.0f);
+    // The definition rounds this product to fp32, then to fp16.  Left alone, the compiler takes both in one mixed-precision
+    // instruction with a single rounding: another scale in one of some 8000 groups.
+    asm volatile("" : "+v"(step));
+    const f16 s = (f16)step;
+    const f16 z = (f16)lo;
     const float sf = (float)s, zf = (float)z;
     const float inv = sf > 0.f ? 1.0f / sf : 0.f;
     c0 = c1 = 0;

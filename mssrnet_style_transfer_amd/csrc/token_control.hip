@@ -71,6 +71,7 @@ __device__ __forceinline__ void tc_store_pick(const TokenControlArgs& a, int64_t
 
 template <typename T>
 __global__ __launch_bounds__(256) void token_control_kernel(TokenControlArgs a) {
+#pragma clang fp contract(off)
     extern __shared__ uint32_t mark[];
     __shared__ unsigned long long best[4];
     const int64_t b = blockIdx.x / (uint32_t)a.chunks;
@@ -120,11 +121,11 @@ __global__ __launch_bounds__(256) void token_control_kernel(TokenControlArgs a) 
             if (mk) {
                 y = y > 0.f ? y / rep : y * rep;
                 const uint32_t c = mk & TC_COUNT;
-                y = __fsub_rn(y, __fadd_rn(__fmul_rn(freq, (float)c), c ? pres : 0.f));
+                y = y - (freq * (float)c + (c ? pres : 0.f));
                 banned |= (mk & TC_BANNED) != 0;
             }
         }
-        if (bias) y = __fadd_rn(y, bias[i]);
+        if (bias) y = y + bias[i];
         const int64_t v = v0 + i;
         if (mask) banned |= !((mask[v >> 5] >> (v & 31)) & 1u);
         if (banned) y = -INFINITY;

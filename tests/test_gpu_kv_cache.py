@@ -175,6 +175,21 @@ def test_extreme_values(kv):
             assert torch.equal(got.nan_to_num(1e30), values(k[:, :, :n]).float().nan_to_num(1e30))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_every_rounding_of_many_groups(kv, dtype):
+    """Half a million groups: a scale rounded once instead of twice shows in one of some 8000."""
+    k, v = heads(8, 8, 2048, 64, dtype, 17, 2.0), heads(8, 8, 2048, 64, dtype, 18)
+    c = kv.KVCache4(8, 8, 64, 2048)
+    c.write(k, v)
+    for got, x in zip(c.read(0, 2048), (k, v)):
+        assert torch.equal(got, values(x).float())
+    few = kv.KVCache4(8 * 2048, 8, 64, 1)                           # the same tokens, one a sentence
+    one = lambda x: x.transpose(1, 2).reshape(8 * 2048, 1, 8, 64).transpose(1, 2)              # noqa: E731
+    few.write(one(k), one(v))
+    for got, x in zip(few.read(0, 1), (one(k), one(v))):
+        assert torch.equal(got, values(x).float())
+
+
 def test_rounding_is_within_half_a_step(kv):
     x = heads(2, 2, 70, 64, torch.float32, 9, 3.0)
     c = kv.KVCache4(2, 2, 64, 70)
