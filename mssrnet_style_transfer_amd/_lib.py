@@ -239,6 +239,11 @@ def stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+def raw_stream(index):
+    """The current stream of device ``index`` as stream() gives it, without building a torch.cuda.Stream (2.7 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def require_cuda(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:

@@ -8,7 +8,6 @@ reference keeps 32.  Tokens are quantised once, when they are written; ``attenti
 These are decoding operators: they build no graph and refuse inputs that would need one.
 """
 import ctypes
-import math
 
 import torch
 
@@ -17,27 +16,30 @@ from . import _lib as L
 MAX_DIM = 128
 
 
-def _no_graph(who, *tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError("%s builds no graph: call it under torch.no_grad()" % who)
+_INTS = (torch.int32, torch.int64)
 
 
-def _rows(who, name, x, B, H, dh):
-    """A [B, H, T, dh] operand with contiguous features, in any order of the other three."""
-    if x.dim() != 4 or x.shape[0] != B or x.shape[1] != H or x.shape[3] != dh:
-        raise ValueError("%s: %s [%d, %d, T, %d] expected (got %s)" % (who, name, B, H, dh, tuple(x.shape)))
-    return x if x.stride(3) == 1 else x.contiguous()
+def _needs_graph(who):
+    raise RuntimeError("%s builds no graph: call it under torch.no_grad()" % who)
 
 
 def _index(who, name, t, B, device):
     """-> (tensor or None, scalar, is int64) of an int or of an integer tensor [B] on the device."""
-    if not torch.is_tensor(t):
+    if not isinstance(t, torch.Tensor):
         return None, int(t), 0
-    if t.shape != (B,) or t.dtype not in (torch.int32, torch.int64) or t.device != device:
+    dtype = t.dtype
+    if t.shape != (B,) or dtype not in _INTS or t.device != device:
         raise ValueError("%s: %s must be an int or an int32 / int64 tensor [%d] on %s (got %s %s on %s)" % (
-            who, name, B, device, t.dtype, tuple(t.shape), t.device))
-    t = t.contiguous()
-    return t, 0, int(t.dtype == torch.int64)
+            who, name, B, device, dtype, tuple(t.shape), t.device))
+    return (t if t.is_contiguous() else t.contiguous()), 0, int(dtype is torch.int64)
+
+
+def _launch(device, fn, *args):
+    """fn(*args, stream) on the device's current stream; the device is made current for the call where it is not."""
+    if device.index == torch.cuda.current_device():
+        return fn(*args, L.raw_stream(device.index))
+    with torch.cuda.device(device):
+        return fn(*args, L.raw_stream(device.index))
 
 
 class KVCache4:
@@ -52,6 +54,7 @@ class KVCache4:
             raise ValueError("KVCache4: %s sentences x %s heads x %s tokens x %s features (a multiple of 8 up to %d)" % (
                 batch, heads, capacity, dim, MAX_DIM))
         self.heads, self.dim, self.capacity = int(heads), int(dim), int(capacity)
+        self._held = None
         # [sentence, bytes]: map() reorders whole sentences
         self.data = torch.zeros(int(batch), n // int(batch), dtype=torch.uint8, device=device)
         L.require_cuda(self.data)
@@ -69,18 +72,30 @@ class KVCache4:
         return self.data.numel()
 
     def _desc(self):
-        return L.Kv4Cache(self.data.data_ptr(), self.batch, self.capacity, self.heads, self.dim)
+        """byref of the C descriptor of the present data."""
+        if self._held is None or self._held[0] is not self.data:
+            d = L.Kv4Cache(self.data.data_ptr(), self.batch, self.capacity, self.heads, self.dim)
+            self._held = (self.data, d, ctypes.byref(d))
+        return self._held[2]
 
     def _span(self, who, start, T, counts):
-        start, start0, wide = _index(who, "start", start, self.batch, self.device)
-        if start is None and not 0 <= start0 <= self.capacity - T:
+        B, device = self.batch, self.device
+        start, start0, wide = _index(who, "start", start, B, device)
+        if T > self.capacity or (start is None and not 0 <= start0 <= self.capacity - T):
             raise ValueError("%s: tokens %d .. %d of a cache of %d" % (who, start0, start0 + T, self.capacity))
-        if T > self.capacity:
-            raise ValueError("%s: %d tokens, the cache holds %d" % (who, T, self.capacity))
-        if counts is not None and not torch.is_tensor(counts):
-            raise ValueError("%s: counts must be an integer tensor [%d] or None" % (who, self.batch))
-        counts, _, wide_c = (None, 0, 0) if counts is None else _index(who, "counts", counts, self.batch, self.device)
+        if counts is None:
+            return start, start0, None, wide
+        if not isinstance(counts, torch.Tensor):
+            raise ValueError("%s: counts must be an integer tensor [%d] or None" % (who, B))
+        counts, _, wide_c = _index(who, "counts", counts, B, device)
         return start, start0, counts, wide | (wide_c << 1)
+
+    def _rows(self, who, name, x):
+        shape = x.shape
+        if len(shape) != 4 or shape[0] != self.batch or shape[1] != self.heads or shape[3] != self.dim:
+            raise ValueError("%s: %s [%d, %d, T, %d] expected (got %s)" % (who, name, self.batch, self.heads, self.dim,
+                                                                         tuple(shape)))
+        return x if x.stride(3) == 1 else x.contiguous()
 
     def write(self, k, v, start=0, counts=None):
         """Quantises k, v [B, heads, T, dim] (float32 or bfloat16, any strides) to positions ``start`` + 0 .. T - 1.
@@ -90,21 +105,22 @@ class KVCache4:
         ``start`` is a tensor and refused where it is an int.  A group of 32 features that holds a NaN or an infinity reads
         back as NaN; values beyond +-65504 are clamped to that."""
         who = "KVCache4.write"
-        _no_graph(who, k, v)
-        L.require_cuda(k, v)
-        k, v = (_rows(who, n, x, self.batch, self.heads, self.dim) for n, x in (("k", k), ("v", v)))
-        T = k.shape[2]
-        if v.shape[2] != T or k.dtype != v.dtype or k.device != self.device or v.device != self.device:
+        if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+            _needs_graph(who)
+        if not (k.is_cuda and v.is_cuda):
+            L.require_cuda(k, v)
+        k, v = self._rows(who, "k", k), self._rows(who, "v", v)
+        device, T = self.device, k.shape[2]
+        if v.shape[2] != T or k.dtype != v.dtype or k.device != device or v.device != device:
             raise ValueError("%s: k and v differ in length, type or device (%s %s %s, %s %s %s; the cache is on %s)" % (
-                who, tuple(k.shape), k.dtype, k.device, tuple(v.shape), v.dtype, v.device, self.device))
+                who, tuple(k.shape), k.dtype, k.device, tuple(v.shape), v.dtype, v.device, device))
         start, start0, counts, bits = self._span(who, start, T, counts)
         if self.batch == 0:
             return
-        with torch.cuda.device(self.device):
-            d = self._desc()
-            L.check(L.load().mssr_kv4_write(ctypes.byref(d), k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-                                            v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), T, L.ptr(start), start0,
-                                            L.ptr(counts), bits, L.dt(k), L.stream()), "kv4_write")
+        kb, kh, kt, _ = k.stride()
+        vb, vh, vt, _ = v.stride()
+        L.check(_launch(device, L.load().mssr_kv4_write, self._desc(), k.data_ptr(), kb, kh, kt, v.data_ptr(), vb, vh, vt, T,
+                        L.ptr(start), start0, L.ptr(counts), bits, L.dt(k)), "kv4_write")
 
     def read(self, start, length, counts=None, dtype=torch.float32):
         """(k, v), each [B, heads, length, dim] (a view of [B, length, heads, dim] memory), of positions ``start`` + 0 ..
@@ -113,15 +129,15 @@ class KVCache4:
         if T < 0:
             raise ValueError("%s: length %d" % (who, T))
         start, start0, counts, bits = self._span(who, start, T, counts)
-        k, v = (torch.empty(self.batch, T, self.heads, self.dim, dtype=dtype, device=self.device).transpose(1, 2)
-                for _ in "kv")
-        if self.batch == 0:
+        B, H, dh = self.batch, self.heads, self.dim
+        # one allocation for both: [2, B, T, H, dh]
+        both = torch.empty_strided((2, B, H, T, dh), (B * T * H * dh, T * H * dh, dh, H * dh, 1), dtype=dtype,
+                                   device=self.device)
+        k, v = both.unbind(0)
+        if B == 0:
             return k, v
-        with torch.cuda.device(self.device):
-            d = self._desc()
-            L.check(L.load().mssr_kv4_read(ctypes.byref(d), k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-                                           v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), T, L.ptr(start), start0,
-                                           L.ptr(counts), bits, L.dt(k), L.stream()), "kv4_read")
+        L.check(_launch(self.device, L.load().mssr_kv4_read, self._desc(), k.data_ptr(), T * H * dh, dh, H * dh, v.data_ptr(),
+                        T * H * dh, dh, H * dh, T, L.ptr(start), start0, L.ptr(counts), bits, L.dt(k)), "kv4_read")
         return k, v
 
     def map(self, fn):
@@ -139,30 +155,33 @@ def attention(q, cache, lengths, scale=None, causal=False, longest=0):
     capacity (it shapes the launch, nothing else).  Returns [B, H, T, dim], a view of [B, T, H, dim] memory, in q's type;
     probabilities are not returned."""
     who = "kv_cache.attention"
-    _no_graph(who, q)
-    L.require_cuda(q)
-    if q.dim() != 4 or q.shape[1] % cache.heads or q.shape[1] == 0:
-        raise ValueError("%s: q [%d, n * %d, T, %d] expected (got %s)" % (who, cache.batch, cache.heads, cache.dim,
-                                                                        tuple(q.shape)))
-    if q.device != cache.device:
-        raise ValueError("%s: q is on %s, the cache on %s" % (who, q.device, cache.device))
-    B, H, T, dh = q.shape
-    q = _rows(who, "q", q, cache.batch, H, cache.dim)
-    lengths, n, wide = _index(who, "lengths", lengths, B, q.device)
-    if lengths is None and not 0 <= n <= cache.capacity:
-        raise ValueError("%s: %d tokens of a cache of %d" % (who, n, cache.capacity))
-    scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
-    out = torch.empty(B, T, H, dh, dtype=q.dtype, device=q.device).transpose(1, 2)
+    if q.requires_grad and torch.is_grad_enabled():
+        _needs_graph(who)
+    if not q.is_cuda:
+        L.require_cuda(q)
+    device, shape, dh = cache.device, q.shape, cache.dim
+    if len(shape) != 4 or shape[0] != cache.batch or shape[3] != dh or shape[1] % cache.heads or shape[1] == 0:
+        raise ValueError("%s: q [%d, n * %d, T, %d] expected (got %s)" % (who, cache.batch, cache.heads, dh, tuple(shape)))
+    if q.device != device:
+        raise ValueError("%s: q is on %s, the cache on %s" % (who, q.device, device))
+    B, H, T, _ = shape
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    lengths, n, wide = _index(who, "lengths", lengths, B, device)
+    if lengths is None:
+        longest = n
+        if not 0 <= n <= cache.capacity:
+            raise ValueError("%s: %d tokens of a cache of %d" % (who, n, cache.capacity))
     code = L.dt(q)
-    lib, d = L.load(), cache._desc()
-    longest = int(longest) if lengths is not None else n
+    out = torch.empty_strided((B, H, T, dh), (T * H * dh, dh, H * dh, 1), dtype=q.dtype, device=device)
     if T == 0 or B == 0:
         return out
-    with torch.cuda.device(q.device):
-        need = lib.mssr_kv4_attention_scratch(ctypes.byref(d), T, H, longest, code)
-        # from the allocator, per call: a call's scratch is its own on every stream and in every captured graph
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-        L.check(lib.mssr_kv4_attention(ctypes.byref(d), q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), out.data_ptr(),
-                                       out.stride(0), out.stride(1), out.stride(2), H, T, L.ptr(lengths), n, wide, longest,
-                                       scale, int(bool(causal)), L.ptr(ws), max(need, 0), code, L.stream()), "kv4_attention")
+    lib, d = L.load(), cache._desc()
+    need = lib.mssr_kv4_attention_scratch(d, T, H, longest, code)
+    # from the allocator, per call: a call's scratch is its own on every stream and in every captured graph
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+    qb, qh, qt, _ = q.stride()
+    L.check(_launch(device, lib.mssr_kv4_attention, d, q.data_ptr(), qb, qh, qt, out.data_ptr(), T * H * dh, dh, H * dh, H, T,
+                    L.ptr(lengths), n, wide, longest, dh ** -0.5 if scale is None else scale, 1 if causal else 0, L.ptr(ws),
+                    need, code), "kv4_attention")
     return out

@@ -46,6 +46,9 @@ class TokenControl:
                             pick(self.state, vec))
 
 
+_NO_RULES = TokenControl()
+
+
 def pack_allowed(allowed):
     """Bool [S, V] -> the int32 words [S, (V + 31) // 32] that ``TokenControl.allowed`` takes."""
     if allowed.dim() != 2 or allowed.dtype != torch.bool:
@@ -56,97 +59,109 @@ def pack_allowed(allowed):
     return torch.where(words >= 1 << 31, words - (1 << 32), words).int()
 
 
-def _ids(who, name, t, shape, device):
-    if t is None:
-        return None, 0
-    if not torch.is_tensor(t) or t.dim() != len(shape) or any(s not in (None, n) for s, n in zip(shape, t.shape)) \
-            or t.dtype not in (torch.int32, torch.int64) or t.device != device:
-        raise ValueError("%s: %s must be an int32 / int64 tensor %s on %s" % (
-            who, name, [s if s is not None else "T" for s in shape], device))
-    return t, int(t.dtype == torch.int64)
+_INTS = (torch.int32, torch.int64)
 
 
-def _f32(who, name, t, shapes, device):
-    if t.dtype != torch.float32 or t.device != device or tuple(t.shape) not in shapes:
-        raise ValueError("%s: %s must be a float32 tensor %s on %s (got %s %s on %s)" % (
-            who, name, " or ".join(map(str, map(list, shapes))), device, t.dtype, tuple(t.shape), t.device))
-    return t
+def _int_error(who, name, shape, device):
+    raise ValueError("%s: %s must be an int32 / int64 tensor %s on %s" % (who, name, shape, device))
+
+
+def _vector(who, name, t, B, device):
+    """-> (contiguous integer tensor [B], its element is 64 bits wide)."""
+    if not isinstance(t, torch.Tensor) or t.shape != (B,) or t.dtype not in _INTS or t.device != device:
+        _int_error(who, name, "[%d]" % B, device)
+    return (t if t.is_contiguous() else t.contiguous()), t.dtype is torch.int64
+
+
+def _rate(who, name, x, B, device):
+    """-> (tensor or None, number) of a penalty."""
+    if not isinstance(x, torch.Tensor):
+        return None, float(x)
+    if x.shape != (B,) or x.dtype != torch.float32 or x.device != device:
+        raise ValueError("%s: %s must be a number or a float32 tensor [%d] on %s (got %s %s on %s)" % (
+            who, name, B, device, x.dtype, tuple(x.shape), x.device))
+    return (x if x.is_contiguous() else x.contiguous()), 0.0
 
 
 def _call(who, logits, control, history, lengths, prompt_lengths, out, ids, empty):
-    if torch.is_grad_enabled() and logits.requires_grad:
+    """Checks, then one call; every tensor made on the way is a local and lives until it is launched."""
+    if logits.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("%s builds no graph: call it under torch.no_grad()" % who)
-    L.require_cuda(logits)
+    if not logits.is_cuda:
+        L.require_cuda(logits)
     if logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError("%s: logits [B, V] expected (got %s)" % (who, tuple(logits.shape)))
     B, V = logits.shape
     dev = logits.device
-    if V > 1 and logits.stride(1) != 1 or B > 1 and logits.stride(0) < V:
+    if not logits.is_contiguous() and (V > 1 and logits.stride(1) != 1 or B > 1 and logits.stride(0) < V):
         logits = logits.contiguous()
-    c = TokenControl() if control is None else control
-    d = L.TokenControlDesc()
-    keep = []                                    # operands made here live until the launch
-
-    def hold(t):
-        keep.append(t)
-        return t.data_ptr()
-
-    d.logits, d.B, d.V, d.ld, d.dtype = logits.data_ptr(), B, V, (logits.stride(0) if B > 1 else V), L.dt(logits)
-    bits = 0
+    c = _NO_RULES if control is None else control
+    bits = h_bs = h_ts = T = bias_bs = states = mode = 0
     if history is not None:
-        history, wide = _ids(who, "history", history, (B, None), dev)
-        bits |= wide
-        d.history, d.h_bs, d.h_ts, d.T = history.data_ptr(), history.stride(0), history.stride(1), history.shape[1]
-    for name, t, bit in (("lengths", lengths, 2), ("prompt_lengths", prompt_lengths, 4)):
-        t, wide = _ids(who, name, t, (B,), dev)
-        if t is not None:
-            if history is None:
-                raise ValueError("%s: %s without a history" % (who, name))
-            setattr(d, name, hold(t.contiguous()))
-            bits |= bit * wide
-    for name in ("repetition", "frequency", "presence"):
-        t = getattr(c, name)
-        if torch.is_tensor(t):
-            setattr(d, name, hold(_f32(who, name, t, ((B,),), dev).contiguous()))
-        else:
-            setattr(d, name + "0", float(t))
-    if c.ngram < 0 or c.ngram > 64:
+        if not isinstance(history, torch.Tensor) or history.dim() != 2 or history.shape[0] != B or \
+                history.dtype not in _INTS or history.device != dev:
+            _int_error(who, "history", "[%d, T]" % B, dev)
+        bits = int(history.dtype is torch.int64)
+        h_bs, h_ts = history.stride()
+        T = history.shape[1]
+        if lengths is not None:
+            lengths, wide = _vector(who, "lengths", lengths, B, dev)
+            bits |= 2 * wide
+        if prompt_lengths is not None:
+            prompt_lengths, wide = _vector(who, "prompt_lengths", prompt_lengths, B, dev)
+            bits |= 4 * wide
+    elif lengths is not None or prompt_lengths is not None:
+        raise ValueError("%s: lengths without a history" % who)
+    rep, rep0 = _rate(who, "repetition", c.repetition, B, dev)
+    freq, freq0 = _rate(who, "frequency", c.frequency, B, dev)
+    pres, pres0 = _rate(who, "presence", c.presence, B, dev)
+    if not 0 <= c.ngram <= 64:
         raise ValueError("%s: ngram %d (0 = none, up to 64)" % (who, c.ngram))
-    d.ngram = int(c.ngram)
-    if c.bias is not None:
-        t = _f32(who, "bias", c.bias, ((V,), (B, V)), dev)
-        if t.stride(-1) != 1 and V > 1:
-            t = t.contiguous()
-        d.bias, d.bias_bs = hold(t), (t.stride(0) if t.dim() == 2 and B > 1 else 0)
-    if c.state is not None and c.allowed is None:
-        raise ValueError("%s: a state without a table of allowed words" % who)
-    if c.allowed is not None:
-        W = (V + 31) // 32
-        t, _ = _ids(who, "allowed", c.allowed, (None, W), dev)
-        if t.dtype != torch.int32 or t.shape[0] < 1:
-            raise ValueError("%s: allowed must be int32 [S, %d]" % (who, W))
-        S = t.shape[0]
-        d.allowed, d.states = hold(t.contiguous()), S
-        if c.state is not None:
-            t, wide = _ids(who, "state", c.state, (B,), dev)
-            d.state, d.state_mode = hold(t.contiguous()), 2
+    bias, allowed, state = c.bias, c.allowed, c.state
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias.device != dev or tuple(bias.shape) not in ((V,), (B, V)):
+            raise ValueError("%s: bias must be a float32 tensor [%d] or [%d, %d] on %s (got %s %s on %s)" % (
+                who, V, B, V, dev, bias.dtype, tuple(bias.shape), bias.device))
+        if bias.stride(-1) != 1:
+            bias = bias.contiguous()
+        if bias.dim() == 2:
+            bias_bs = bias.stride(0)
+    if allowed is not None:
+        states = allowed.shape[0]
+        if allowed.dim() != 2 or allowed.shape[1] != (V + 31) // 32 or states < 1 or allowed.dtype != torch.int32 or \
+                allowed.device != dev:
+            raise ValueError("%s: allowed must be an int32 tensor [S, %d] on %s" % (who, (V + 31) // 32, dev))
+        if not allowed.is_contiguous():
+            allowed = allowed.contiguous()
+        if state is not None:
+            state, wide = _vector(who, "state", state, B, dev)
+            mode = 2
             bits |= 8 * wide
-        elif S in (1, B):
-            d.state_mode = 0 if S == 1 else 1
-        else:
-            raise ValueError("%s: %d rows of allowed words for %d sentences need a state" % (who, S, B))
-    if out is not None:
-        d.out, d.ldo = out.data_ptr(), (out.stride(0) if B > 1 else V)
-    with torch.cuda.device(dev):
-        lib = L.load()
-        if ids is not None:
-            d.ids, d.empty = ids.data_ptr(), int(empty)
-            bits |= 16 * int(ids.dtype == torch.int64)
-            need = lib.mssr_token_control_scratch(max(B, 1), V)
-            if need > 0:                         # a call's own: streams and captured graphs share none
-                d.scratch, d.scratch_bytes = hold(torch.empty(need, dtype=torch.uint8, device=dev)), need
-        d.index_bits = bits
-        L.check(lib.mssr_token_control(ctypes.byref(d), L.stream()), "token_control")
+        elif states == B:
+            mode = 1
+        elif states != 1:
+            raise ValueError("%s: %d rows of allowed words for %d sentences need a state" % (who, states, B))
+    elif state is not None:
+        raise ValueError("%s: a state without a table of allowed words" % who)
+    code = L.dt(logits)
+    if B == 0:
+        return
+    lib, ptr, ws, need = L.load(), L.ptr, None, 0
+    if ids is not None:
+        bits |= 16 * int(ids.dtype is torch.int64)
+        need = lib.mssr_token_control_scratch(B, V)
+        if need > 0:                             # a call's own: streams and captured graphs share none
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    d = L.TokenControlDesc(logits.data_ptr(), ptr(out), B, V, logits.stride(0) if B > 1 else V,
+                           0 if out is None else (out.stride(0) if B > 1 else V), ptr(history), h_bs, h_ts, T, ptr(lengths),
+                           ptr(prompt_lengths), ptr(rep), ptr(freq), ptr(pres), rep0, freq0, pres0, int(c.ngram), ptr(bias),
+                           bias_bs, ptr(allowed), states, ptr(state), mode, ptr(ids), int(empty), bits, code, ptr(ws), need)
+    if dev.index == torch.cuda.current_device():
+        rc = lib.mssr_token_control(ctypes.byref(d), L.raw_stream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = lib.mssr_token_control(ctypes.byref(d), L.raw_stream(dev.index))
+    L.check(rc, "token_control")
 
 
 def control_logits(logits, control=None, history=None, lengths=None, prompt_lengths=None, out=None):
