@@ -12,7 +12,7 @@
 // 16-byte loads and 8 codes become an 8-element operand with one shift and four ANDs (see kv4_attention.hip):
 //   K: lane (quad, n) holds, for token 16 t + n and group g, features 32 g + 8 quad + 0..7 in dword t * NG + g;
 //      feature 2 r sits in nibble r, feature 2 r + 1 in nibble r + 4
-//   V: lane (quad, n) holds, for tokens 32 ks + 8 quad + 4 h + 0..3 (one byte each) of dword (ks * NG + g) * 2 + h,
+//   V: lane (quad, n) holds, for tokens 32 ks + 16 h + 4 quad + 0..3 (one byte each) of dword (ks * NG + g) * 2 + h,
 //      feature 32 g + n in the low and feature 32 g + 16 + n in the high nibble
 // and dword d of lane l is at (d / 4) * 1024 + l * 16 + (d % 4) * 4.  A token owns whole bytes in both, so tokens are
 // written without reading their neighbours.
@@ -48,8 +48,8 @@ __device__ __forceinline__ int kv4_k_off(int ng, int tok, int g, int quad) {
 }
 // byte of (token, group g, n); n + 1 is 16 bytes further
 __device__ __forceinline__ int kv4_v_off(int ng, int tok, int g, int n) {
-    const int d = ((tok >> 5) * ng + g) * 2 + ((tok >> 2) & 1);
-    return ng * 1024 + (d >> 2) * 1024 + (((tok >> 3) & 3) * 16 + n) * 16 + (d & 3) * 4 + (tok & 3);
+    const int d = ((tok >> 5) * ng + g) * 2 + ((tok >> 4) & 1);
+    return ng * 1024 + (d >> 2) * 1024 + (((tok >> 2) & 3) * 16 + n) * 16 + (d & 3) * 4 + (tok & 3);
 }
 __device__ __forceinline__ int kv4_kmeta_off(int ng, int tok, int g) { return ng * 2048 + (tok * ng + g) * 4; }
 __device__ __forceinline__ int kv4_vmeta_off(int ng, int tok, int g) { return ng * 2304 + (tok * ng + g) * 4; }

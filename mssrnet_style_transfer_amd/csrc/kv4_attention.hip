@@ -6,18 +6,16 @@
 // so the matrix instructions take the CODES as they lie and the scales touch only scores and probabilities: one number
 // a token instead of 32.  A code needs no conversion: the bit pattern of an integer c < 256 read as bf16 is the number
 // c * 2^-133 (subnormals, which the matrix cores keep), so `x & 0x000f000f` IS an operand pair, `x & 0x00f000f0` one
-// that is 16 times as large; the other operand carries 2^64 (q) or 2^96 (p s) so that every product is a normal fp32
-// number, and powers of two cost nothing in precision.  8 codes take 5 vector instructions.
+// that is 16 times as large; the other operand (q, or p s) carries 2^64 so that every product is a normal fp32 number,
+// and powers of two cost nothing in precision.  8 codes take 5 vector instructions.
 //
-// A wave takes 64 tokens at a time, one token a lane from the scores on:
-//   scores  4 products of 16 tokens x 32 features per group (mfma 16x16x32), accumulated into ONE result: the q operand
-//           of product t is zero but for rows 4 t .. 4 t + 3, so lane (quad, n) ends with the scores of token
-//           16 quad + n = its own number, for up to four query rows
-//   softmax one token a lane; the running maximum moves only when a score passes it by more than 8 (then every sum is
-//           rescaled), so that a block of tokens costs one comparison and no cross-lane reduction
-//   p s     in bf16 parts (2 for bf16 queries: 2^-17 of p; 3 for fp32), transposed through 2 to 3 KB of LDS a group
-//   context 2 products of 32 tokens per 16 features
-// fp32 queries go in as three bf16 parts in three rows: one query row where bf16 ones have four.
+// A number enters a product as bf16 parts whose products add up in fp32: bf16 queries are one part, fp32 ones three (all
+// 24 bits); p s, an fp32 number, two for bf16 results (2^-17 of it is lost, 2^-8 of the result is rounded away) and three
+// for fp32 ones.
+//
+// A wave takes 64 tokens at a time; the running maximum moves only when a score passes it by more than 8 (then every
+// sum is rescaled), so that a block of tokens costs one comparison and no cross-lane reduction.  The W waves of a block
+// take every W-th 64 tokens of its share of the sentence and are joined through LDS; a second launch joins the shares.
 #include "kv4.hpp"
 
 namespace mssr {
@@ -37,12 +35,9 @@ struct Kv4AttnArgs {
     int64_t rows;                   // B * Hkv * NQ
 };
 
-constexpr float KV4_QUP = 0x1p64f, KV4_PUP = 0x1p96f;
-constexpr float KV4_SDOWN = 0x1p69f, KV4_ODOWN = 0x1p37f;      // 2^133 over the above
-
-__device__ __forceinline__ float kv4_bf_lo(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
-__device__ __forceinline__ float kv4_bf_hi(uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
-__device__ __forceinline__ uint16_t kv4_bf_bits(float x) { return __builtin_bit_cast(uint16_t, (bf16)x); }
+constexpr float KV4_UP = 0x1p64f, KV4_DOWN = 0x1p69f;          // UP * DOWN * 2^-133 = 1
+constexpr float KV4_LAZY = 8.f;                                // log2 of how far a probability may pass 1 before a rescale
+constexpr int KV4_UPLOG = 64;
 
 // 8 codes of a K dword -> operand whose elements 2 r, 2 r + 1 are features 2 r, 2 r + 1 (r odd: times 16)
 __device__ __forceinline__ bf16x8 kv4_k_operand(uint32_t x) {
@@ -50,13 +45,17 @@ __device__ __forceinline__ bf16x8 kv4_k_operand(uint32_t x) {
     u32x4 r = {x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u};
     return __builtin_bit_cast(bf16x8, r);
 }
-// two V dwords (8 tokens) -> operands of feature n and of feature 16 + n (times 16); token order 0 2 1 3 4 6 5 7
+// two V dwords (4 tokens of tile 2 ks, 4 of tile 2 ks + 1) -> operands of feature n and of feature 16 + n (times 16);
+// the four tokens of a dword come in the order 0 2 1 3
 __device__ __forceinline__ void kv4_v_operands(uint32_t x0, uint32_t x1, bf16x8& lo, bf16x8& hi) {
     const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
     u32x4 l = {x0 & 0x000f000fu, y0 & 0x000f000fu, x1 & 0x000f000fu, y1 & 0x000f000fu};
     u32x4 h = {x0 & 0x00f000f0u, y0 & 0x00f000f0u, x1 & 0x00f000f0u, y1 & 0x00f000f0u};
     lo = __builtin_bit_cast(bf16x8, l);
     hi = __builtin_bit_cast(bf16x8, h);
+}
+__device__ __forceinline__ f32x4 kv4_mfma(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
 template <int NG>
@@ -73,265 +72,442 @@ struct Kv4Tile {            // a lane's share of a block: 16 NG bytes of K codes
     }
 };
 
-// T: query type.  NG: groups of 32 features.  RS: row sets (of 4 bf16 query rows or 1 fp32 one) a block works on.
-// W: waves; wave w takes every W-th block of the split.
-template <typename T, int NG, int RS, int W>
-__global__ __launch_bounds__(64 * W) void kv4_attention_kernel(Kv4AttnArgs a) {
+struct Kv4Work {            // what a block works on: query rows q0 .. of (sentence, key/value head), blocks [first, last)
+    int64_t b, bh, len, first, last;
+    int hk, q0, split;
+    __device__ __forceinline__ Kv4Work(const Kv4AttnArgs& a, int rows) {
+        const uint32_t chunks = (a.NQ + rows - 1) / rows;
+        uint32_t id = blockIdx.x;
+        split = id % a.splits;
+        id /= a.splits;
+        q0 = (int)(id % chunks) * rows;
+        bh = id / chunks;
+        b = bh / a.Hkv;
+        hk = (int)(bh % a.Hkv);
+        len = a.lengths.at(b);
+        len = len < 0 ? 0 : (len > a.capacity ? a.capacity : len);
+        const int64_t nb = (len + KV4_TOK - 1) / KV4_TOK, per = (nb + a.splits - 1) / a.splits;
+        first = split * per;
+        last = first + per < nb ? first + per : nb;
+    }
+};
+
+// 8 features of a query row as bf16 parts times 2^64 (elements that meet a code times 16: 2^60); returns their sum
+template <typename T, int PARTS>
+__device__ __forceinline__ float kv4_query(const T* src, bool on, bf16x8 (&op)[PARTS]) {
+    float x[8] = {};
+    if (on) {
+        if constexpr (sizeof(T) == 4) {
+            __builtin_memcpy(x, src, 32);
+        } else {
+            bf16x8 v;
+            __builtin_memcpy(&v, src, 16);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = (float)v[e];
+        }
+    }
+    const float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float y = x[e];
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            const bf16 h = (bf16)y;
+            y -= (float)h;
+            op[p][e] = (bf16)((float)h * (((e >> 1) & 1) ? KV4_UP / 16.f : KV4_UP));
+        }
+    }
+    return sum;
+}
+
+// Joins the block's waves (om: per wave and row the context, maximum and sum; synchronised by the caller) and writes the
+// row, or its share of it.
+template <typename T, int W, int R, int DP>
+__device__ __forceinline__ void kv4_finish(const Kv4AttnArgs& a, const Kv4Work& wk, const float (&om)[W][R][DP + 4]) {
+    for (int x = threadIdx.x; x < R * (DP / 2); x += 64 * W) {
+        const int r = x / (DP / 2), c = x % (DP / 2) * 2, qi = wk.q0 + r;
+        if (qi >= a.NQ || c >= a.dh) continue;
+        float top = om[0][r][DP], sum = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+        for (int k = 1; k < W; ++k) top = fmaxf(top, om[k][r][DP]);
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            const float mk = om[k][r][DP], lk = om[k][r][DP + 1];
+            // a wave that saw nothing has nothing to add (its maximum is minus infinity, like the joint one may be)
+            const float f = mk == -INFINITY && lk == 0.f ? 0.f : __builtin_amdgcn_exp2f(mk - top);
+            sum = fmaf(f, lk, sum);
+            o0 = fmaf(f, om[k][r][c], o0);
+            o1 = fmaf(f, om[k][r][c + 1], o1);
+        }
+        if (a.splits == 1) {
+            const int i = qi % a.Tq, h = wk.hk * a.G + qi / a.Tq;
+            T* dst = (T*)a.out + wk.b * a.o_bs + h * a.o_hs + i * a.o_ts + c;
+            dst[0] = from_f<T>(sum == 0.f ? 0.f : o0 / sum);
+            dst[1] = from_f<T>(sum == 0.f ? 0.f : o1 / sum);
+        } else {
+            const int64_t at = (wk.bh * a.NQ + qi) * a.splits + wk.split;
+            a.part[at * a.dh + c] = o0;
+            a.part[at * a.dh + c + 1] = o1;
+            if (c == 0) {
+                float* ml = a.part + a.rows * a.splits * a.dh + at * 2;
+                ml[0] = top;
+                ml[1] = sum;
+            }
+        }
+    }
+}
+
+// Up to 4 query rows (R of them in use) of a key/value head: the decode step.  One token a lane from the scores on.
+//   scores   per group 4 products of 16 tokens; every quad of rows of the q operand holds the same rows, so lane
+//            (quad, n) finds token n of each product and keeps the one of its own 16 (one fp32 row: its 3 parts are rows)
+//   p s      goes through LDS to become an operand: row 4 part + r, the parts add up at the end
+// Bound by the cache's bytes: at 64 features about 130 vector and 16 matrix instructions for 5 KB.
+template <typename T, int NG, int R, int W>
+__global__ __launch_bounds__(64 * W) void kv4_few_kernel(Kv4AttnArgs a) {
     constexpr bool F32 = sizeof(T) == 4;
-    constexpr int R = F32 ? 1 : 4;               // query rows of a row set
-    constexpr int PARTS = F32 ? 3 : 2;           // bf16 parts of p s
+    constexpr bool QROWS = F32 && R == 1;        // the parts of q in rows of one product instead of products of their own
+    constexpr int QP = F32 ? 3 : 1, PP = F32 ? 3 : 2;
     constexpr int PLD = 72;                      // bf16 elements of an LDS row of 64 tokens: 16-byte reads of 16 rows spread
     constexpr int DP = NG * 32;
-    __shared__ __align__(16) uint16_t ps[W][NG * PARTS * 4][PLD];
-    __shared__ float om[W > 1 ? W : 1][R][DP + 2];
+    __shared__ __align__(16) uint16_t ps[W][NG][PP * R][PLD];
+    __shared__ float om[W][R][DP + 4];
 
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, quad = lane >> 4;
-    const int chunks = (a.NQ + RS * R - 1) / (RS * R);
-    uint32_t id = blockIdx.x;
-    const int split = id % a.splits;
-    id /= a.splits;
-    const int q0 = (int)(id % chunks) * (RS * R);
-    const uint32_t bh = id / chunks;
-    const int64_t b = bh / a.Hkv;
-    const int hk = bh % a.Hkv;
-
-    int64_t len = a.lengths.at(b);
-    len = len < 0 ? 0 : (len > a.capacity ? a.capacity : len);
-    const int64_t nb = (len + KV4_TOK - 1) / KV4_TOK, per = (nb + a.splits - 1) / a.splits;
-    const int64_t first = split * per, last = first + per < nb ? first + per : nb;
-
-    // query operands: lane (row n of the product, quad): features 32 g + 8 quad + 0..7 of query row 4 rs.. + (n & 3)
-    bf16x8 qop[RS][NG];
-    float qsum[RS][R][NG];                       // scale * sum of q over the group, every lane
-    int64_t lim[RS][R];
-    const T* qrow[RS][R];
-    bool have[RS][R];
-#pragma unroll
-    for (int rs = 0; rs < RS; ++rs)
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int qi = q0 + rs * R + r;
-            have[rs][r] = qi < a.NQ;
-            const int i = have[rs][r] ? qi % a.Tq : 0, h = hk * a.G + (have[rs][r] ? qi / a.Tq : 0);
-            qrow[rs][r] = (const T*)a.q + b * a.q_bs + h * a.q_hs + i * a.q_ts;
-            lim[rs][r] = have[rs][r] ? (a.causal ? len - a.Tq + 1 + i : len) : 0;
-        }
-#pragma unroll
-    for (int rs = 0; rs < RS; ++rs) {
+    const Kv4Work wk(a, R);
+    bf16x8 qop[QROWS ? 1 : QP][NG];
+    float qsum[R][NG];                           // scale * sum of q over the group
+    int64_t lim[R];
+    {
+        const int r = R == 1 ? 0 : (n & 3), qi = wk.q0 + r;
+        const bool have = qi < a.NQ;
+        const int i = have ? qi % a.Tq : 0, h = wk.hk * a.G + (have ? qi / a.Tq : 0);
+        const T* src = (const T*)a.q + wk.b * a.q_bs + h * a.q_hs + i * a.q_ts;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            const int ch = g * 32 + quad * 8, r = F32 ? 0 : (n & 3);
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = 0.f;
-            const T* src = qrow[rs][0];
-            bool on = have[rs][0];
-            if (!F32) {
-#pragma unroll
-                for (int rr = 1; rr < R; ++rr)
-                    if (r == rr) { src = qrow[rs][rr]; on = have[rs][rr]; }
-            }
-            if (on && ch < a.dh) {
-                if constexpr (F32) {
-                    __builtin_memcpy(x, src + ch, 32);
-                } else {
-                    bf16x8 v;
-                    __builtin_memcpy(&v, src + ch, 16);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = (float)v[e];
-                }
-            }
-            float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+            const int ch = g * 32 + quad * 8;
+            bf16x8 op[QP];
+            float sum = kv4_query<T, QP>(src + ch, have && ch < a.dh, op);
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
 #pragma unroll
-            for (int rr = 0; rr < R; ++rr) qsum[rs][rr][g] = lane_read(sum, rr) * a.scale;
-            bf16x8 op;
+            for (int rr = 0; rr < R; ++rr) qsum[rr][g] = lane_read(sum, rr) * a.scale;
+            if constexpr (QROWS) {
+                const bf16x8 none = {};
+                qop[0][g] = (n & 3) == 0 ? op[0] : (n & 3) == 1 ? op[1] : (n & 3) == 2 ? op[2] : none;
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                float y = x[e];
-                if (F32) {                       // rows 0, 1, 2 of a quad: the three parts
-                    const bf16 p0 = (bf16)y;
-                    const float y1 = y - (float)p0;
-                    const bf16 p1 = (bf16)y1;
-                    const float y2 = y1 - (float)p1;
-                    y = (n & 3) == 0 ? (float)p0 : (n & 3) == 1 ? (float)p1 : (n & 3) == 2 ? y2 : 0.f;
-                }
-                op[e] = (bf16)(y * (((e >> 1) & 1) ? KV4_QUP / 16.f : KV4_QUP));
+                for (int p = 0; p < QP; ++p) qop[p][g] = op[p];
             }
-            qop[rs][g] = op;
+        }
+#pragma unroll
+        for (int rr = 0; rr < R; ++rr) {
+            const int k = wk.q0 + rr;
+            lim[rr] = k < a.NQ ? (a.causal ? wk.len - a.Tq + 1 + k % a.Tq : wk.len) : 0;
         }
     }
 
-    float m[RS][R], l[RS][R], zs[RS][R][NG];
-    f32x4 acc[RS][2 * NG];
+    float m[R], l[R], zs[R][NG];                 // m: the reference of the exponents, 64 below the running maximum's
+    f32x4 acc[2 * NG];
 #pragma unroll
-    for (int rs = 0; rs < RS; ++rs) {
+    for (int r = 0; r < R; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            m[rs][r] = -INFINITY;
-            l[rs][r] = 0.f;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) zs[rs][r][g] = 0.f;
-        }
-#pragma unroll
-        for (int c = 0; c < 2 * NG; ++c) acc[rs][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int g = 0; g < NG; ++g) zs[r][g] = 0.f;
     }
-    const uint8_t* base = a.data + (int64_t)bh * a.blocks * kv4_block_bytes(NG);
-    const bf16x8 zero8 = {};
+#pragma unroll
+    for (int c = 0; c < 2 * NG; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const uint8_t* base = a.data + wk.bh * a.blocks * kv4_block_bytes(NG);
+    const float down = KV4_DOWN * a.scale;
+    // where this lane's token goes among the operand's 64: half, quad, then 0 2 1 3
+    const int col = (lane & 32) | ((lane & 12) << 1) | ((lane & 16) >> 2) | ((lane & 1) << 1) | ((lane >> 1) & 1);
+    const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
 
     Kv4Tile<NG> cur, nxt;
-    if (first + w < last) cur.load(base + (first + w) * kv4_block_bytes(NG), lane);
-    for (int64_t blk = first + w; blk < last; blk += W) {
-        const bool more = blk + W < last;
+    if (wk.first + w < wk.last) cur.load(base + (wk.first + w) * kv4_block_bytes(NG), lane);
+    for (int64_t blk = wk.first + w; blk < wk.last; blk += W) {
+        const bool more = blk + W < wk.last;
         if (more) nxt.load(base + (blk + W) * kv4_block_bytes(NG), lane);
         const int64_t tok = blk * KV4_TOK + lane;
-        // ---- scores
-        f32x4 sc[RS][NG];
-#pragma unroll
-        for (int rs = 0; rs < RS; ++rs)
-#pragma unroll
-            for (int g = 0; g < NG; ++g) sc[rs][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const bf16x8 kop = kv4_k_operand(cur.k[(t * NG + g) >> 2][(t * NG + g) & 3]);
-#pragma unroll
-                for (int rs = 0; rs < RS; ++rs) {
-                    const bf16x8 qt = (n >> 2) == t ? qop[rs][g] : zero8;
-                    sc[rs][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qt, kop, sc[rs][g], 0, 0, 0);
-                }
-            }
-        float ksc[NG], kz[NG], vsc[NG], vz[NG];
+        uint32_t mk[NG], mv[NG];
 #pragma unroll
         for (int g = 0; g < NG; ++g) {           // past the sentence's end the cache may hold anything
-            const uint32_t mk = tok < len ? cur.mk[g] : 0u, mv = tok < len ? cur.mv[g] : 0u;
-            ksc[g] = kv4_scale(mk) * (KV4_SDOWN * a.scale);
-            kz[g] = kv4_zero(mk);
-            vsc[g] = kv4_scale(mv) * KV4_PUP;
-            vz[g] = kv4_zero(mv);
+            mk[g] = tok < wk.len ? cur.mk[g] : 0u;
+            mv[g] = tok < wk.len ? cur.mv[g] : 0u;
         }
-        bf16x8 vop[2][2 * NG];
+        float dot[R], off[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) dot[r] = off[r] = 0.f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            f32x4 d[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const bf16x8 kop = kv4_k_operand(cur.k[(t * NG + g) >> 2][(t * NG + g) & 3]);
+                d[t] = kv4_mfma(qop[0][g], kop, zero4);
+                if constexpr (!QROWS) {
+#pragma unroll
+                    for (int p = 1; p < QP; ++p) d[t] = kv4_mfma(qop[p][g], kop, d[t]);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float x = quad == 0 ? d[0][r] : quad == 1 ? d[1][r] : quad == 2 ? d[2][r] : d[3][r];
+                if constexpr (QROWS) {
+                    x += (quad == 0 ? d[0][1] : quad == 1 ? d[1][1] : quad == 2 ? d[2][1] : d[3][1]) +
+                         (quad == 0 ? d[0][2] : quad == 1 ? d[1][2] : quad == 2 ? d[2][2] : d[3][2]);
+                }
+                dot[r] = fmaf(x, kv4_scale(mk[g]), dot[r]);
+                off[r] = fmaf(qsum[r][g], kv4_zero(mk[g]), off[r]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const bool see = tok < lim[r];
+            const float s = see ? fmaf(dot[r], down, off[r]) : -INFINITY;
+            if (__any(s - KV4_UPLOG > m[r] + KV4_LAZY)) {
+                const float mn = wave_max(s) - KV4_UPLOG, f = __builtin_amdgcn_exp2f(m[r] - mn);
+                m[r] = mn;
+                l[r] *= f;
+#pragma unroll
+                for (int g = 0; g < NG; ++g) zs[r][g] *= f;
+#pragma unroll
+                for (int c = 0; c < 2 * NG; ++c) acc[c][r] *= f;
+            }
+            const float p = see ? __builtin_amdgcn_exp2f(s - m[r]) : 0.f;
+            l[r] += p;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                float y = see ? p * kv4_scale(mv[g]) : 0.f;
+                zs[r][g] += see ? p * kv4_zero(mv[g]) : 0.f;
+#pragma unroll
+                for (int part = 0; part < PP; ++part) {
+                    const bf16 h = (bf16)y;
+                    y -= (float)h;
+                    ps[w][g][part * R + r][col] = __builtin_bit_cast(uint16_t, h);
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        // rows 4 part + r; the rows of absent parts and queries repeat others and are not used
+        const int row = R == 1 ? ((n >> 2) < PP ? (n >> 2) : 0) : ((n >> 2) < PP ? n : (n & 3));
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 const int d = (ks * NG + g) * 2;
-                kv4_v_operands(cur.v[d >> 2][d & 3], cur.v[d >> 2][(d & 3) + 1], vop[ks][2 * g], vop[ks][2 * g + 1]);
+                bf16x8 lo, hi;
+                kv4_v_operands(cur.v[d >> 2][d & 3], cur.v[d >> 2][(d & 3) + 1], lo, hi);
+                const u32x4 raw = *reinterpret_cast<const u32x4*>(&ps[w][g][row][ks * 32 + quad * 8]);
+                const bf16x8 pop = __builtin_bit_cast(bf16x8, raw);
+                acc[2 * g] = kv4_mfma(pop, lo, acc[2 * g]);
+                acc[2 * g + 1] = kv4_mfma(pop, hi, acc[2 * g + 1]);
             }
-#pragma unroll
-        for (int rs = 0; rs < RS; ++rs) {
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                float s = 0.f;
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const float dot = F32 ? sc[rs][g][0] + (sc[rs][g][1] + sc[rs][g][2]) : sc[rs][g][r];
-                    s = fmaf(dot, ksc[g], s);
-                    s = fmaf(qsum[rs][r][g], kz[g], s);
-                }
-                const bool see = tok < lim[rs][r];
-                s = see ? s : -INFINITY;
-                if (__any(s > m[rs][r] + 8.f)) {
-                    const float mn = wave_max(s), f = __builtin_amdgcn_exp2f(m[rs][r] - mn);
-                    m[rs][r] = mn;
-                    l[rs][r] *= f;
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) zs[rs][r][g] *= f;
-#pragma unroll
-                    for (int c = 0; c < 2 * NG; ++c) {
-                        if (F32) acc[rs][c] *= f;
-                        else acc[rs][c][r] *= f;
-                    }
-                }
-                const float p = see ? __builtin_amdgcn_exp2f(s - m[rs][r]) : 0.f;
-                l[rs][r] += p;
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    float y = see ? p * vsc[g] : 0.f;
-                    zs[rs][r][g] += see ? p * vz[g] : 0.f;
-                    // tokens 1 and 2 of four change places: the order of kv4_v_operands
-                    const int col = (lane & ~3) | ((lane & 1) << 1) | ((lane >> 1) & 1);
-#pragma unroll
-                    for (int part = 0; part < PARTS; ++part) {
-                        const bf16 h = (bf16)y;
-                        y -= (float)h;
-                        ps[w][(g * PARTS + part) * 4 + r][col] = __builtin_bit_cast(uint16_t, h);
-                    }
-                }
-            }
-            __builtin_amdgcn_wave_barrier();
-            // ---- context: row 4 part + r of the product; rows of absent parts repeat others and are not used
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const int row = (n >> 2) < PARTS ? n : (n & 3);
-                    const u32x4 raw = *reinterpret_cast<const u32x4*>(&ps[w][g * PARTS * 4 + row][ks * 32 + quad * 8]);
-                    const bf16x8 pop = __builtin_bit_cast(bf16x8, raw);
-                    acc[rs][2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pop, vop[ks][2 * g], acc[rs][2 * g], 0, 0, 0);
-                    acc[rs][2 * g + 1] =
-                        __builtin_amdgcn_mfma_f32_16x16x32_bf16(pop, vop[ks][2 * g + 1], acc[rs][2 * g + 1], 0, 0, 0);
-                }
-            __builtin_amdgcn_wave_barrier();
-        }
+        __builtin_amdgcn_wave_barrier();
         if (more) cur = nxt;
     }
 
-    // ---- sums over lanes, then over the block's waves
 #pragma unroll
-    for (int rs = 0; rs < RS; ++rs) {
-        if (W > 1 && rs) __syncthreads();
+    for (int r = 0; r < R; ++r) {
+        const float lt = wave_sum(l[r]) * (1.f / KV4_UP);
+        float zt[NG];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const float lt = wave_sum(l[rs][r]);
-            float zt[NG];
+        for (int g = 0; g < NG; ++g) zt[g] = wave_sum(zs[r][g]) * (1.f / KV4_UP);
 #pragma unroll
-            for (int g = 0; g < NG; ++g) zt[g] = wave_sum(zs[rs][r][g]);
+        for (int c = 0; c < 2 * NG; ++c) {
+            const float v = acc[c][r];
+            float u = v + __shfl_xor(v, 16);                    // parts 0 + 1 (quads 0 and 1)
+            if (PP == 3) u += __shfl_xor(v, 32);                // quad 0: + part 2
+            u = fmaf(u, (c & 1) ? KV4_DOWN / 16.f : KV4_DOWN, zt[c >> 1]);
+            if (quad == 0) om[w][r][c * 16 + n] = u;
+        }
+        if (lane == 0) {
+            om[w][r][DP] = m[r];
+            om[w][r][DP + 1] = lt;
+        }
+    }
+    if (W > 1) __syncthreads();
+    else __builtin_amdgcn_wave_barrier();
+    kv4_finish<T, W, R, DP>(a, wk, om);
+}
+
+// 16 query rows of a key/value head: shared heads, several new tokens.  One query row a lane, 16 of the block's 64 tokens
+// in each quad of lanes, everything transposed:
+//   scores   tokens x queries: lane (quad, n) holds tokens 16 t + 4 quad + 0..3 of query n
+//   p s      is an operand as it lies (slots 0-3 from tile 2 ks, 4-7 from 2 ks + 1, the order of the V codes)
+//   context  features x queries: lane (quad, n) holds features 16 c + 4 quad + 0..3 of query n
+// The (s, z) pairs are one a token and reach the lanes through LDS.
+template <typename T, int NG, int W>
+__global__ __launch_bounds__(64 * W) void kv4_many_kernel(Kv4AttnArgs a) {
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int QP = F32 ? 3 : 1, PP = F32 ? 3 : 2;
+    constexpr int DP = NG * 32;
+    __shared__ __align__(16) uint32_t meta[W][2][KV4_TOK * NG];
+    __shared__ float om[W][16][DP + 4];
+
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, quad = lane >> 4;
+    const Kv4Work wk(a, 16);
+    bf16x8 qop[QP][NG];
+    float qsum[NG];
+    const int qi = wk.q0 + n;
+    const bool have = qi < a.NQ;
+    const int64_t lim = have ? (a.causal ? wk.len - a.Tq + 1 + qi % a.Tq : wk.len) : 0;
+    // every row of the block sees at least this many tokens: blocks below it need no comparisons
+    const int64_t sure = a.causal ? wk.len - a.Tq + 1 : wk.len;
+    {
+        const int i = have ? qi % a.Tq : 0, h = wk.hk * a.G + (have ? qi / a.Tq : 0);
+        const T* src = (const T*)a.q + wk.b * a.q_bs + h * a.q_hs + i * a.q_ts;
 #pragma unroll
-            for (int c = 0; c < 2 * NG; ++c) {
-                float v = acc[rs][c][r];
-                float u = v + __shfl_xor(v, 16);                    // parts 0 + 1 (quads 0 and 1)
-                if (PARTS == 3) u += __shfl_xor(v, 32);             // quad 0: + part 2
-                u = fmaf(u, (c & 1) ? KV4_ODOWN / 16.f : KV4_ODOWN, zt[c >> 1]);
-                if (quad == 0) om[w][r][c * 16 + n] = u;
+        for (int g = 0; g < NG; ++g) {
+            const int ch = g * 32 + quad * 8;
+            bf16x8 op[QP];
+            float sum = kv4_query<T, QP>(src + ch, have && ch < a.dh, op);
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            qsum[g] = sum * a.scale;
+#pragma unroll
+            for (int p = 0; p < QP; ++p) qop[p][g] = op[p];
+        }
+    }
+    float m = -INFINITY, l = 0.f, zs[NG];
+    f32x4 acc[2 * NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) zs[g] = 0.f;
+#pragma unroll
+    for (int c = 0; c < 2 * NG; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const uint8_t* base = a.data + wk.bh * a.blocks * kv4_block_bytes(NG);
+    const float down = KV4_DOWN * a.scale;
+    const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
+
+    Kv4Tile<NG> cur, nxt;
+    if (wk.first + w < wk.last) cur.load(base + (wk.first + w) * kv4_block_bytes(NG), lane);
+    for (int64_t blk = wk.first + w; blk < wk.last; blk += W) {
+        const bool more = blk + W < wk.last;
+        if (more) nxt.load(base + (blk + W) * kv4_block_bytes(NG), lane);
+        const bool edge = (blk + 1) * KV4_TOK > sure;
+        const int64_t left = lim - blk * KV4_TOK, kept = wk.len - blk * KV4_TOK;
+        const int see = (int)(left > KV4_TOK ? KV4_TOK : left);      // tokens of this block that the row sees
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            meta[w][0][lane * NG + g] = lane < kept ? cur.mk[g] : 0u;
+            meta[w][1][lane * NG + g] = lane < kept ? cur.mv[g] : 0u;
+        }
+        __builtin_amdgcn_wave_barrier();
+        float s[4][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            f32x4 d[NG];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const bf16x8 kop = kv4_k_operand(cur.k[(t * NG + g) >> 2][(t * NG + g) & 3]);
+                d[g] = kv4_mfma(kop, qop[0][g], zero4);
+#pragma unroll
+                for (int p = 1; p < QP; ++p) d[g] = kv4_mfma(kop, qop[p][g], d[g]);
             }
-            if (lane == 0) {
-                om[w][r][DP] = m[rs][r];
-                om[w][r][DP + 1] = lt;
+            uint32_t mk[4 * NG];
+            __builtin_memcpy(mk, __builtin_assume_aligned(&meta[w][0][(16 * t + 4 * quad) * NG], 16), 16 * NG);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float dot = 0.f, off = 0.f;
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    dot = fmaf(d[g][r], kv4_scale(mk[r * NG + g]), dot);
+                    off = fmaf(qsum[g], kv4_zero(mk[r * NG + g]), off);
+                }
+                s[t][r] = fmaf(dot, down, off);
             }
         }
-        if (W > 1) __syncthreads();
-        else __builtin_amdgcn_wave_barrier();
-        for (int x = threadIdx.x; x < R * DP; x += 64 * W) {
-            const int r = x / DP, c = x % DP, qi = q0 + rs * R + r;
-            if (qi >= a.NQ || c >= a.dh) continue;
-            float top = om[0][r][DP], sum = 0.f, o = 0.f;
+        if (edge) {
 #pragma unroll
-            for (int k = 1; k < W; ++k) top = fmaxf(top, om[k][r][DP]);
+            for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int k = 0; k < W; ++k) {
-                const float mk = om[k][r][DP];
-                // a wave that saw nothing has nothing to add (and its maximum is minus infinity)
-                const float f = mk == -INFINITY && om[k][r][DP + 1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(mk - top);
-                sum = fmaf(f, om[k][r][DP + 1], sum);
-                o = fmaf(f, om[k][r][c], o);
+                for (int r = 0; r < 4; ++r) s[t][r] = 16 * t + 4 * quad + r < see ? s[t][r] : -INFINITY;
+        }
+        float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+#pragma unroll
+        for (int t = 1; t < 4; ++t) top = fmaxf(top, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
+        if (__any(top - KV4_UPLOG > m + KV4_LAZY)) {
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float mn = fmaxf(m, top - KV4_UPLOG);
+            const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) zs[g] *= f;
+#pragma unroll
+            for (int c = 0; c < 2 * NG; ++c) acc[c] *= f;
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const bool on = !edge || 16 * t + 4 * quad + r < see;
+                s[t][r] = on ? __builtin_amdgcn_exp2f(s[t][r] - m) : 0.f;
+                l += s[t][r];
             }
-            if (a.splits == 1) {
-                const int i = qi % a.Tq, h = hk * a.G + qi / a.Tq;
-                ((T*)a.out)[b * a.o_bs + h * a.o_hs + i * a.o_ts + c] = from_f<T>(sum == 0.f ? 0.f : o / sum);
-            } else {
-                const int64_t row = (int64_t)bh * a.NQ + qi, at = row * a.splits + split;
-                a.part[at * a.dh + c] = o;
-                if (c == 0) {
-                    float* ml = a.part + a.rows * a.splits * a.dh + at * 2;
-                    ml[0] = top;
-                    ml[1] = sum;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            uint32_t mv[2][4 * NG];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                __builtin_memcpy(mv[h], __builtin_assume_aligned(&meta[w][1][(32 * ks + 16 * h + 4 * quad) * NG], 16), 16 * NG);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                bf16x8 pop[PP];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = (j >> 1) | ((j & 1) << 1), t = 2 * ks + h;            // order 0 2 1 3
+                        const float p = s[t][r];
+                        const bool on = !edge || 16 * t + 4 * quad + r < see;
+                        float y = p * kv4_scale(mv[h][r * NG + g]);
+                        float z = p * kv4_zero(mv[h][r * NG + g]);
+                        if (edge) { y = on ? y : 0.f; z = on ? z : 0.f; }
+                        zs[g] += z;
+#pragma unroll
+                        for (int part = 0; part < PP; ++part) {
+                            const bf16 b = (bf16)y;
+                            y -= (float)b;
+                            pop[part][4 * h + j] = b;
+                        }
+                    }
+                const int d = (ks * NG + g) * 2;
+                bf16x8 lo, hi;
+                kv4_v_operands(cur.v[d >> 2][d & 3], cur.v[d >> 2][(d & 3) + 1], lo, hi);
+#pragma unroll
+                for (int part = 0; part < PP; ++part) {
+                    acc[2 * g] = kv4_mfma(lo, pop[part], acc[2 * g]);
+                    acc[2 * g + 1] = kv4_mfma(hi, pop[part], acc[2 * g + 1]);
                 }
             }
         }
+        __builtin_amdgcn_wave_barrier();
+        if (more) cur = nxt;
     }
+
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        float z = zs[g];
+        z += __shfl_xor(z, 16);
+        z += __shfl_xor(z, 32);
+        z *= 1.f / KV4_UP;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                om[w][n][g * 32 + h * 16 + quad * 4 + r] = fmaf(acc[2 * g + h][r], h ? KV4_DOWN / 16.f : KV4_DOWN, z);
+    }
+    if (quad == 0) {
+        om[w][n][DP] = m;
+        om[w][n][DP + 1] = l * (1.f / KV4_UP);
+    }
+    if (W > 1) __syncthreads();
+    else __builtin_amdgcn_wave_barrier();
+    kv4_finish<T, W, 16, DP>(a, wk, om);
 }
 
 // joins the splits of a query row: one wave a row
@@ -360,15 +536,13 @@ __global__ __launch_bounds__(64) void kv4_join_kernel(Kv4AttnArgs a) {
     if (c1 < a.dh) dst[c1] = from_f<T>(sum == 0.f ? 0.f : o1 / sum);
 }
 
-struct Kv4Shape { int RS, W, splits; int64_t units, chunks; };
+struct Kv4Shape { int rows, W, splits; int64_t units; };
 
 // How a call is cut: `longest` bounds the lengths (the capacity where the caller knows no better).
-static Kv4Shape kv4_shape(int64_t B, int Hkv, int NQ, int dtype, int64_t longest) {
+static Kv4Shape kv4_shape(int64_t B, int Hkv, int NQ, int64_t longest) {
     Kv4Shape s;
-    const int R = dtype == MSSR_F32 ? 1 : 4;
-    s.RS = NQ > R ? 2 : 1;
-    s.chunks = (NQ + s.RS * R - 1) / (s.RS * R);
-    s.units = B * Hkv * s.chunks;
+    s.rows = NQ == 1 ? 1 : NQ <= 4 ? 4 : 16;
+    s.units = B * Hkv * ((NQ + s.rows - 1) / s.rows);
     const int64_t nb = (longest + KV4_TOK - 1) / KV4_TOK;
     s.W = nb <= 1 || s.units >= 4096 ? 1 : 4;
     const int64_t want = 4096 / (s.units * s.W), most = (nb + s.W - 1) / s.W;
@@ -377,18 +551,19 @@ static Kv4Shape kv4_shape(int64_t B, int Hkv, int NQ, int dtype, int64_t longest
     return s;
 }
 
-template <typename T, int NG, int RS>
+template <typename T, int NG, int W>
 static void kv4_launch(const Kv4AttnArgs& a, const Kv4Shape& s, hipStream_t st) {
     const unsigned grid = (unsigned)(s.units * s.splits);
-    if (s.W == 1) kv4_attention_kernel<T, NG, RS, 1><<<grid, 64, 0, st>>>(a);
-    else kv4_attention_kernel<T, NG, RS, 4><<<grid, 256, 0, st>>>(a);
+    if (s.rows == 1) kv4_few_kernel<T, NG, 1, W><<<grid, 64 * W, 0, st>>>(a);
+    else if (s.rows == 4) kv4_few_kernel<T, NG, 4, W><<<grid, 64 * W, 0, st>>>(a);
+    else kv4_many_kernel<T, NG, W><<<grid, 64 * W, 0, st>>>(a);
 }
 template <typename T>
 static void kv4_dispatch(const Kv4AttnArgs& a, const Kv4Shape& s, int ng, hipStream_t st) {
-#define MSSR_KV4_A(NG)                                  \
-    case NG:                                            \
-        if (s.RS == 1) kv4_launch<T, NG, 1>(a, s, st);  \
-        else kv4_launch<T, NG, 2>(a, s, st);            \
+#define MSSR_KV4_A(NG)                                \
+    case NG:                                          \
+        if (s.W == 1) kv4_launch<T, NG, 1>(a, s, st); \
+        else kv4_launch<T, NG, 4>(a, s, st);          \
         break;
     switch (ng) { MSSR_KV4_A(1) MSSR_KV4_A(2) MSSR_KV4_A(3) MSSR_KV4_A(4) }
 #undef MSSR_KV4_A
@@ -407,7 +582,7 @@ extern "C" int64_t mssr_kv4_attention_scratch(const mssr_kv4_cache* c, int64_t T
     if (!c || c->B < 1 || c->H < 1 || H < c->H || H % c->H || Tq < 1 || c->capacity < 1 || !valid_dtype(dtype)) return -1;
     if (Tq > INT32_MAX / (H / c->H)) return -1;
     const int NQ = (int)(H / c->H * Tq);
-    const Kv4Shape s = kv4_shape(c->B, c->H, NQ, dtype, kv4_longest(c, longest));
+    const Kv4Shape s = kv4_shape(c->B, c->H, NQ, kv4_longest(c, longest));
     return s.splits > 1 ? c->B * c->H * NQ * s.splits * (c->dh + 2) * (int64_t)sizeof(float) : 0;
 }
 
@@ -426,7 +601,7 @@ extern "C" int mssr_kv4_attention(const mssr_kv4_cache* c, const void* q, int64_
     if (Tq == 0) return MSSR_OK;
     MSSR_REQUIRE(Tq <= (INT32_MAX >> 8) / (H / c->H), "kv4_attention: %lld query rows", (long long)Tq);
     const int NQ = (int)(H / c->H * Tq);
-    const Kv4Shape s = kv4_shape(c->B, c->H, NQ, dtype, kv4_longest(c, longest));
+    const Kv4Shape s = kv4_shape(c->B, c->H, NQ, kv4_longest(c, longest));
     const int64_t rows = c->B * c->H * NQ;
     MSSR_REQUIRE(s.units <= KV4_MAX_GRID / s.splits && rows <= KV4_MAX_GRID, "kv4_attention: %lld query rows in one call",
                  (long long)rows);

@@ -206,7 +206,7 @@ __global__ __launch_bounds__(256) void kv4_write_blocks_kernel(Kv4WriteArgs a, u
             lo = (d / NG) * 16 + ((i >> 2) & 15);
         } else if (i < NG * 512) {                      // V codes: four tokens, a byte each
             const int q = i - NG * 256, d = (q >> 8) * 4 + (q & 3);
-            lo = (d / (2 * NG)) * 32 + ((q >> 6) & 3) * 8 + (d & 1) * 4;
+            lo = (d / (2 * NG)) * 32 + (d & 1) * 16 + ((q >> 6) & 3) * 4;
             n = 4;
         } else {
             lo = ((i - NG * 512) / NG) & (KV4_TOK - 1); // (s, z) pairs: K's 64 tokens, then V's
