@@ -4,19 +4,21 @@
 //   q . k_t = sum_g s_tg (sum_{c in g} q_c code_tc) + z_tg (sum_{c in g} q_c)
 //   o_c     = (sum_t (p_t s_tg) code_tc + sum_t p_t z_tg) / sum_t p_t
 // so the matrix instructions take the CODES as they lie and the scales touch only scores and probabilities: one number
-// a token instead of 32.  A code needs no conversion: the bit pattern of an integer c < 256 read as bf16 is the number
-// c * 2^-133 (subnormals, which the matrix cores keep), so `x & 0x000f000f` IS an operand pair, `x & 0x00f000f0` one
-// that is 16 times as large; the other operand (q, or p s) carries 2^64 so that every product is a normal fp32 number,
-// and powers of two cost nothing in precision.  8 codes take 5 vector instructions.
+// a token instead of 32.  A code needs no conversion: the bit pattern of an integer c < 1024 read as fp16 is the number
+// c * 2^-24 (subnormals, which the matrix cores keep), so `x & 0x000f000f` IS an operand pair and `x & 0x00f000f0` one
+// that is 16 times as large.  8 codes take 5 vector instructions.
 //
-// A number enters a product as bf16 parts whose products add up in fp32: bf16 queries are one part, fp32 ones three (all
-// 24 bits); p s, an fp32 number, two for bf16 results (2^-17 of it is lost, 2^-8 of the result is rounded away) and three
-// for fp32 ones.
+// What meets the codes is fp16 too (11 bits), as parts whose products add up in fp32: one part for bf16 calls (exact for
+// q; 2^-11 of p s, averaged over tokens, where the result keeps 2^-8), two for fp32 ones (2^-22).  Powers of two keep
+// them in fp16's range: a query row is scaled to a largest element in [2^13, 2^14); p s is taken relative to the largest
+// V scale met so far (rounded up to a power of two; when it grows, the sums shrink), with p up to 2^8 (below) and 7 bits
+// on top, so that what is 2^-21 of the largest still has all its bits and the rest is off by at most 2^-32 of it.
 //
 // A wave takes 64 tokens at a time; the running maximum moves only when a score passes it by more than 8 (then every
 // sum is rescaled), so that a block of tokens costs one comparison and no cross-lane reduction.  The W waves of a block
 // take every W-th 64 tokens of its share of the sentence and are joined through LDS; a second launch joins the shares.
 #include "kv4.hpp"
+#include <type_traits>
 
 namespace mssr {
 
@@ -33,98 +35,138 @@ struct Kv4AttnArgs {
     float scale;                    // of the scores, times log2(e)
     float* part;                    // [rows][splits][dh] unnormalised context, then [rows][splits][2] (max, sum)
     int64_t rows;                   // B * Hkv * NQ
+    uint32_t units;                 // pieces of work: B * Hkv * chunks of query rows * splits
 };
 
-constexpr float KV4_UP = 0x1p64f, KV4_DOWN = 0x1p69f;          // UP * DOWN * 2^-133 = 1
-constexpr float KV4_LAZY = 8.f;                                // log2 of how far a probability may pass 1 before a rescale
-constexpr int KV4_UPLOG = 64;
+constexpr float KV4_LAZY = 8.f;          // log2 of how far a probability may pass 1 before a rescale
+constexpr float KV4_UP = 7.f;            // log2 of what probabilities are held times
+constexpr float KV4_NONE = -3e38f;       // the reference of a row that has seen no token: 2^(-inf - KV4_NONE) is 0
+constexpr int KV4_MAX_SPLITS = 512;
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // 8 codes of a K dword -> operand whose elements 2 r, 2 r + 1 are features 2 r, 2 r + 1 (r odd: times 16)
-__device__ __forceinline__ bf16x8 kv4_k_operand(uint32_t x) {
+__device__ __forceinline__ f16x8 kv4_k_operand(uint32_t x) {
     const uint32_t y = x >> 8;
     u32x4 r = {x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u};
-    return __builtin_bit_cast(bf16x8, r);
+    return __builtin_bit_cast(f16x8, r);
 }
 // two V dwords (4 tokens of tile 2 ks, 4 of tile 2 ks + 1) -> operands of feature n and of feature 16 + n (times 16);
 // the four tokens of a dword come in the order 0 2 1 3
-__device__ __forceinline__ void kv4_v_operands(uint32_t x0, uint32_t x1, bf16x8& lo, bf16x8& hi) {
+__device__ __forceinline__ void kv4_v_operands(uint32_t x0, uint32_t x1, f16x8& lo, f16x8& hi) {
     const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
     u32x4 l = {x0 & 0x000f000fu, y0 & 0x000f000fu, x1 & 0x000f000fu, y1 & 0x000f000fu};
     u32x4 h = {x0 & 0x00f000f0u, y0 & 0x00f000f0u, x1 & 0x00f000f0u, y1 & 0x00f000f0u};
-    lo = __builtin_bit_cast(bf16x8, l);
-    hi = __builtin_bit_cast(bf16x8, h);
+    lo = __builtin_bit_cast(f16x8, l);
+    hi = __builtin_bit_cast(f16x8, h);
 }
-__device__ __forceinline__ f32x4 kv4_mfma(bf16x8 a, bf16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+__device__ __forceinline__ f32x4 kv4_mfma(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+// the product of this lane's quad, by two conditions (four nested ones become branches)
+__device__ __forceinline__ float kv4_own(float a, float b, float c, float d, bool odd, bool upper) {
+    const float lo = odd ? b : a, hi = odd ? d : c;
+    return upper ? hi : lo;
+}
+
+// A lane's share of a block: 16 NG bytes of K codes, of V codes, and its token's (s, z) pairs.  The next block's K half is
+// requested when the scores have used this one's, its V half when the context has: no second set of registers.
 template <int NG>
-struct Kv4Tile {            // a lane's share of a block: 16 NG bytes of K codes, of V codes, and its token's (s, z) pairs
+struct Kv4Tile {
     u32x4 k[NG], v[NG];
     uint32_t mk[NG], mv[NG];
-    __device__ __forceinline__ void load(const uint8_t* blk, int lane) {
+    __device__ __forceinline__ void load_k(const uint8_t* blk, int lane) {
 #pragma unroll
         for (int i = 0; i < NG; ++i) k[i] = *reinterpret_cast<const u32x4*>(blk + i * 1024 + lane * 16);
         __builtin_memcpy(mk, __builtin_assume_aligned(blk + NG * 2048 + lane * (4 * NG), 4), 4 * NG);
+    }
+    __device__ __forceinline__ void load_v(const uint8_t* blk, int lane) {
+        __builtin_memcpy(mv, __builtin_assume_aligned(blk + NG * 2304 + lane * (4 * NG), 4), 4 * NG);
 #pragma unroll
         for (int i = 0; i < NG; ++i) v[i] = *reinterpret_cast<const u32x4*>(blk + NG * 1024 + i * 1024 + lane * 16);
-        __builtin_memcpy(mv, __builtin_assume_aligned(blk + NG * 2304 + lane * (4 * NG), 4), 4 * NG);
     }
 };
+
+// waves of a block: W work together; of lone ones, four share a block for the sake of the launch (4096 blocks of one wave
+// each take longer to start than to run)
+constexpr int kv4_waves(int W) { return W == 1 ? 4 : W; }
 
 struct Kv4Work {            // what a block works on: query rows q0 .. of (sentence, key/value head), blocks [first, last)
-    int64_t b, bh, len, first, last;
-    int hk, q0, split;
-    __device__ __forceinline__ Kv4Work(const Kv4AttnArgs& a, int rows) {
-        const uint32_t chunks = (a.NQ + rows - 1) / rows;
-        uint32_t id = blockIdx.x;
-        split = id % a.splits;
-        id /= a.splits;
-        q0 = (int)(id % chunks) * rows;
+    int64_t len;
+    uint32_t b, bh;
+    int hk, q0, split, first, last;     // a sentence has fewer than 2^31 blocks (the entry point checks it)
+    __device__ __forceinline__ Kv4Work(const Kv4AttnArgs& a, int rows, uint32_t id) {
+        split = id % (uint32_t)a.splits;
+        id /= (uint32_t)a.splits;
+        const uint32_t chunks = (uint32_t)(a.NQ + rows - 1) / (uint32_t)rows;
         bh = id / chunks;
-        b = bh / a.Hkv;
-        hk = (int)(bh % a.Hkv);
+        q0 = (int)(id - bh * chunks) * rows;
+        b = bh / (uint32_t)a.Hkv;
+        hk = (int)(bh - b * (uint32_t)a.Hkv);
+    }
+    __device__ __forceinline__ void span(const Kv4AttnArgs& a) {
         len = a.lengths.at(b);
         len = len < 0 ? 0 : (len > a.capacity ? a.capacity : len);
-        const int64_t nb = (len + KV4_TOK - 1) / KV4_TOK, per = (nb + a.splits - 1) / a.splits;
-        first = split * per;
-        last = first + per < nb ? first + per : nb;
+        const uint32_t nb = (uint32_t)((len + KV4_TOK - 1) >> 6), per = (nb + (uint32_t)a.splits - 1) / (uint32_t)a.splits;
+        const uint32_t lo = (uint32_t)split * per, hi = lo + per;
+        first = (int)(lo < nb ? lo : nb);
+        last = (int)(hi < nb ? hi : nb);
     }
 };
 
-// 8 features of a query row as bf16 parts times 2^64 (elements that meet a code times 16: 2^60); returns their sum
-template <typename T, int PARTS>
-__device__ __forceinline__ float kv4_query(const T* src, bool on, bf16x8 (&op)[PARTS]) {
-    float x[8] = {};
-    if (on) {
-        if constexpr (sizeof(T) == 4) {
-            __builtin_memcpy(x, src, 32);
-        } else {
-            bf16x8 v;
-            __builtin_memcpy(&v, src, 16);
+// The features of a query row that this lane multiplies (8 of every group), and the row's scaling.
+template <typename T, int NG, int PARTS>
+struct Kv4Query {
+    f16x8 op[PARTS][NG];        // fp16 parts of q * 2^up; where the code is 16 times as large, a 16th
+    float sum[NG];              // sum of q over the group, every lane of the row
+    int up;
+    __device__ __forceinline__ void load(const T* src, bool have, int dh, int quad) {
+        float x[NG][8], top = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = (float)v[e];
+        for (int g = 0; g < NG; ++g) {
+            const int ch = g * 32 + quad * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[g][e] = 0.f;
+            if (have && ch < dh) {
+                if constexpr (sizeof(T) == 4) {
+                    __builtin_memcpy(x[g], src + ch, 32);
+                } else {
+                    bf16x8 v;
+                    __builtin_memcpy(&v, src + ch, 16);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[g][e] = (float)v[e];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[g][e]));
+            float t = ((x[g][0] + x[g][1]) + (x[g][2] + x[g][3])) + ((x[g][4] + x[g][5]) + (x[g][6] + x[g][7]));
+            t += __shfl_xor(t, 16);
+            sum[g] = t + __shfl_xor(t, 32);
         }
-    }
-    const float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        up = top > 0.f ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        float y = x[e];
+        for (int g = 0; g < NG; ++g)
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-            const bf16 h = (bf16)y;
-            y -= (float)h;
-            op[p][e] = (bf16)((float)h * (((e >> 1) & 1) ? KV4_UP / 16.f : KV4_UP));
-        }
+            for (int e = 0; e < 8; ++e) {
+                float y = __builtin_amdgcn_ldexpf(x[g][e], ((e >> 1) & 1) ? up - 4 : up);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    const f16 h = (f16)y;
+                    y -= (float)h;
+                    op[p][g][e] = h;
+                }
+            }
     }
-    return sum;
-}
+};
 
 // Joins the block's waves (om: per wave and row the context, maximum and sum; synchronised by the caller) and writes the
 // row, or its share of it.
 template <typename T, int W, int R, int DP>
 __device__ __forceinline__ void kv4_finish(const Kv4AttnArgs& a, const Kv4Work& wk, const float (&om)[W][R][DP + 4]) {
-    for (int x = threadIdx.x; x < R * (DP / 2); x += 64 * W) {
+    for (int x = W == 1 ? threadIdx.x & 63 : threadIdx.x; x < R * (DP / 2); x += 64 * W) {
         const int r = x / (DP / 2), c = x % (DP / 2) * 2, qi = wk.q0 + r;
         if (qi >= a.NQ || c >= a.dh) continue;
         float top = om[0][r][DP], sum = 0.f, o0 = 0.f, o1 = 0.f;
@@ -141,11 +183,11 @@ __device__ __forceinline__ void kv4_finish(const Kv4AttnArgs& a, const Kv4Work& 
         }
         if (a.splits == 1) {
             const int i = qi % a.Tq, h = wk.hk * a.G + qi / a.Tq;
-            T* dst = (T*)a.out + wk.b * a.o_bs + h * a.o_hs + i * a.o_ts + c;
+            T* dst = (T*)a.out + (int64_t)wk.b * a.o_bs + (int64_t)h * a.o_hs + (int64_t)i * a.o_ts + c;
             dst[0] = from_f<T>(sum == 0.f ? 0.f : o0 / sum);
             dst[1] = from_f<T>(sum == 0.f ? 0.f : o1 / sum);
         } else {
-            const int64_t at = (wk.bh * a.NQ + qi) * a.splits + wk.split;
+            const int64_t at = ((int64_t)wk.bh * a.NQ + qi) * a.splits + wk.split;
             a.part[at * a.dh + c] = o0;
             a.part[at * a.dh + c + 1] = o1;
             if (c == 0) {
@@ -159,81 +201,98 @@ __device__ __forceinline__ void kv4_finish(const Kv4AttnArgs& a, const Kv4Work& 
 
 // Up to 4 query rows (R of them in use) of a key/value head: the decode step.  One token a lane from the scores on.
 //   scores   per group 4 products of 16 tokens; every quad of rows of the q operand holds the same rows, so lane
-//            (quad, n) finds token n of each product and keeps the one of its own 16 (one fp32 row: its 3 parts are rows)
+//            (quad, n) finds token n of each product and keeps the one of its own 16 (one fp32 row: its parts are rows)
 //   p s      goes through LDS to become an operand: row 4 part + r, the parts add up at the end
-// Bound by the cache's bytes: at 64 features about 130 vector and 16 matrix instructions for 5 KB.
 template <typename T, int NG, int R, int W>
-__global__ __launch_bounds__(64 * W) void kv4_few_kernel(Kv4AttnArgs a) {
+__global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnArgs a) {
     constexpr bool F32 = sizeof(T) == 4;
+    constexpr int PARTS = F32 ? 2 : 1;
     constexpr bool QROWS = F32 && R == 1;        // the parts of q in rows of one product instead of products of their own
-    constexpr int QP = F32 ? 3 : 1, PP = F32 ? 3 : 2;
-    constexpr int PLD = 72;                      // bf16 elements of an LDS row of 64 tokens: 16-byte reads of 16 rows spread
+    constexpr int PLD = 72;                      // fp16 elements of an LDS row of 64 tokens: 16-byte reads of 16 rows spread
     constexpr int DP = NG * 32;
-    __shared__ __align__(16) uint16_t ps[W][NG][PP * R][PLD];
-    __shared__ float om[W][R][DP + 4];
+    __shared__ __align__(16) uint16_t ps_[kv4_waves(W)][NG][PARTS * R][PLD];
+    __shared__ float om_[kv4_waves(W) / W][W][R][DP + 4];
 
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, quad = lane >> 4;
-    const Kv4Work wk(a, R);
-    bf16x8 qop[QROWS ? 1 : QP][NG];
-    float qsum[R][NG];                           // scale * sum of q over the group
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = W == 1 ? 0 : wave;
+    const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
+    const uint32_t id = W == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+    if (W == 1 && id >= a.units) return;         // (the waves of such a block never wait for each other)
+    auto& ps = ps_[wave];
+    auto& om = om_[W == 1 ? wave : 0];
+    Kv4Work wk(a, R, id);
+    const uint8_t* base = a.data + (int64_t)wk.bh * a.blocks * kv4_block_bytes(NG);
+    Kv4Tile<NG> cur;
+    const bool early = W == 1 && a.splits == 1;  // a lone wave's first block is known before its length is
+    if (early) {
+        cur.load_k(base, lane);
+        cur.load_v(base, lane);
+    }
+    wk.span(a);
+    f16x8 qop[QROWS ? 1 : PARTS][NG];
+    float qsum[R][NG], down[R];                  // scale * sum of q over the group; what a score's codes' part is scaled by
     int64_t lim[R];
     {
         const int r = R == 1 ? 0 : (n & 3), qi = wk.q0 + r;
         const bool have = qi < a.NQ;
         const int i = have ? qi % a.Tq : 0, h = wk.hk * a.G + (have ? qi / a.Tq : 0);
-        const T* src = (const T*)a.q + wk.b * a.q_bs + h * a.q_hs + i * a.q_ts;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const int ch = g * 32 + quad * 8;
-            bf16x8 op[QP];
-            float sum = kv4_query<T, QP>(src + ch, have && ch < a.dh, op);
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-#pragma unroll
-            for (int rr = 0; rr < R; ++rr) qsum[rr][g] = lane_read(sum, rr) * a.scale;
-            if constexpr (QROWS) {
-                const bf16x8 none = {};
-                qop[0][g] = (n & 3) == 0 ? op[0] : (n & 3) == 1 ? op[1] : (n & 3) == 2 ? op[2] : none;
-            } else {
-#pragma unroll
-                for (int p = 0; p < QP; ++p) qop[p][g] = op[p];
-            }
-        }
+        Kv4Query<T, NG, PARTS> q;
+        q.load((const T*)a.q + (int64_t)wk.b * a.q_bs + (int64_t)h * a.q_hs + (int64_t)i * a.q_ts, have, a.dh, quad);
+        const float back = __builtin_amdgcn_ldexpf(a.scale, 24 - q.up);
 #pragma unroll
         for (int rr = 0; rr < R; ++rr) {
             const int k = wk.q0 + rr;
             lim[rr] = k < a.NQ ? (a.causal ? wk.len - a.Tq + 1 + k % a.Tq : wk.len) : 0;
+            down[rr] = lane_read(back, rr);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) qsum[rr][g] = lane_read(q.sum[g], rr) * a.scale;
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            if constexpr (QROWS) {
+                const f16x8 none = {};
+                qop[0][g] = (n & 3) == 0 ? q.op[0][g] : (n & 3) == 1 ? q.op[PARTS - 1][g] : none;
+            } else {
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) qop[p][g] = q.op[p][g];
+            }
         }
     }
 
-    float m[R], l[R], zs[R][NG];                 // m: the reference of the exponents, 64 below the running maximum's
+    // m: the running maximum (up to 8 behind), ref: what exponents are taken relative to, m - 7 + log2 of the V scales' bound;
+    // every sum of a row is in units of 2^ref, so that nothing but ref remembers either
+    float m[R], ref[R], l[R], zs[R][NG], vtop = 0.f;
     f32x4 acc[2 * NG];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        m[r] = -INFINITY;
+        m[r] = ref[r] = KV4_NONE;
         l[r] = 0.f;
 #pragma unroll
         for (int g = 0; g < NG; ++g) zs[r][g] = 0.f;
     }
 #pragma unroll
     for (int c = 0; c < 2 * NG; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const uint8_t* base = a.data + wk.bh * a.blocks * kv4_block_bytes(NG);
-    const float down = KV4_DOWN * a.scale;
     // where this lane's token goes among the operand's 64: half, quad, then 0 2 1 3
     const int col = (lane & 32) | ((lane & 12) << 1) | ((lane & 16) >> 2) | ((lane & 1) << 1) | ((lane >> 1) & 1);
     const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
+    const bool odd = quad & 1, upper = quad & 2;
 
-    Kv4Tile<NG> cur, nxt;
-    if (wk.first + w < wk.last) cur.load(base + (wk.first + w) * kv4_block_bytes(NG), lane);
-    for (int64_t blk = wk.first + w; blk < wk.last; blk += W) {
+    const uint8_t* ahead = base + (int64_t)(wk.first + w) * kv4_block_bytes(NG);
+    if (!early && wk.first + w < wk.last) {
+        cur.load_k(ahead, lane);
+        cur.load_v(ahead, lane);
+    }
+    for (int blk = wk.first + w; blk < wk.last; blk += W) {
         const bool more = blk + W < wk.last;
-        if (more) nxt.load(base + (blk + W) * kv4_block_bytes(NG), lane);
-        const int64_t tok = blk * KV4_TOK + lane;
+        ahead += W * kv4_block_bytes(NG);
+        const int64_t at = (int64_t)blk * KV4_TOK;
+        const bool kept = lane < wk.len - at;
         uint32_t mk[NG], mv[NG];
+        float top = 0.f;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {           // past the sentence's end the cache may hold anything
-            mk[g] = tok < wk.len ? cur.mk[g] : 0u;
-            mv[g] = tok < wk.len ? cur.mv[g] : 0u;
+            mk[g] = kept ? cur.mk[g] : 0u;
+            mv[g] = kept ? cur.mv[g] : 0u;
+            top = fmaxf(top, kv4_scale(mv[g]));
         }
         float dot[R], off[R];
 #pragma unroll
@@ -243,86 +302,100 @@ __global__ __launch_bounds__(64 * W) void kv4_few_kernel(Kv4AttnArgs a) {
             f32x4 d[4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const bf16x8 kop = kv4_k_operand(cur.k[(t * NG + g) >> 2][(t * NG + g) & 3]);
+                const f16x8 kop = kv4_k_operand(cur.k[(t * NG + g) >> 2][(t * NG + g) & 3]);
                 d[t] = kv4_mfma(qop[0][g], kop, zero4);
-                if constexpr (!QROWS) {
-#pragma unroll
-                    for (int p = 1; p < QP; ++p) d[t] = kv4_mfma(qop[p][g], kop, d[t]);
-                }
+                if constexpr (PARTS == 2 && !QROWS) d[t] = kv4_mfma(qop[PARTS - 1][g], kop, d[t]);
             }
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                float x = quad == 0 ? d[0][r] : quad == 1 ? d[1][r] : quad == 2 ? d[2][r] : d[3][r];
-                if constexpr (QROWS) {
-                    x += (quad == 0 ? d[0][1] : quad == 1 ? d[1][1] : quad == 2 ? d[2][1] : d[3][1]) +
-                         (quad == 0 ? d[0][2] : quad == 1 ? d[1][2] : quad == 2 ? d[2][2] : d[3][2]);
-                }
+                float x = kv4_own(d[0][r], d[1][r], d[2][r], d[3][r], odd, upper);
+                if constexpr (QROWS) x += kv4_own(d[0][1], d[1][1], d[2][1], d[3][1], odd, upper);
                 dot[r] = fmaf(x, kv4_scale(mk[g]), dot[r]);
                 off[r] = fmaf(qsum[r][g], kv4_zero(mk[g]), off[r]);
             }
+            if (R > 1) __builtin_amdgcn_sched_barrier(0);        // a group at a time, for the registers
+        }
+        if (more) cur.load_k(ahead, lane);
+        float s[R];
+        uint32_t mask[R];
+        bool far = top > vtop;                   // NaN scales are passed over: they make their own features NaN and no others
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const bool see = lane < lim[r] - at;
+            s[r] = fmaf(dot[r], down[r], off[r]);
+            s[r] = see ? s[r] : -INFINITY;
+            // one row sees what the sentence has; of several, each may see less, and a NaN that it does not see is not its
+            mask[r] = R == 1 || see ? ~0u : 0u;
+            far |= s[r] > m[r] + KV4_LAZY;
+        }
+        if (__any(far)) {
+            vtop = fmaxf(vtop, wave_max(top));
+            const float e = vtop > 0.f ? (float)__builtin_amdgcn_frexp_expf(vtop) - KV4_UP : 0.f;
+            f32x4 f = {1.f, 1.f, 1.f, 1.f};
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                m[r] = fmaxf(m[r], wave_max(s[r]));
+                const float moved = m[r] + e;
+                f[r] = __builtin_amdgcn_exp2f(ref[r] - moved);
+                ref[r] = moved;
+                l[r] *= f[r];
+#pragma unroll
+                for (int g = 0; g < NG; ++g) zs[r][g] *= f[r];
+            }
+#pragma unroll
+            for (int c = 0; c < 2 * NG; ++c) acc[c] *= f;
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const bool see = tok < lim[r];
-            const float s = see ? fmaf(dot[r], down, off[r]) : -INFINITY;
-            if (__any(s - KV4_UPLOG > m[r] + KV4_LAZY)) {
-                const float mn = wave_max(s) - KV4_UPLOG, f = __builtin_amdgcn_exp2f(m[r] - mn);
-                m[r] = mn;
-                l[r] *= f;
-#pragma unroll
-                for (int g = 0; g < NG; ++g) zs[r][g] *= f;
-#pragma unroll
-                for (int c = 0; c < 2 * NG; ++c) acc[c][r] *= f;
-            }
-            const float p = see ? __builtin_amdgcn_exp2f(s - m[r]) : 0.f;
+            const float p = __builtin_amdgcn_exp2f(s[r] - ref[r]);
             l[r] += p;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                float y = see ? p * kv4_scale(mv[g]) : 0.f;
-                zs[r][g] += see ? p * kv4_zero(mv[g]) : 0.f;
+                const uint32_t mvr = mv[g] & mask[r];
+                float y = p * kv4_scale(mvr);
+                zs[r][g] = fmaf(p, kv4_zero(mvr), zs[r][g]);
 #pragma unroll
-                for (int part = 0; part < PP; ++part) {
-                    const bf16 h = (bf16)y;
+                for (int part = 0; part < PARTS; ++part) {
+                    const f16 h = (f16)y;
                     y -= (float)h;
-                    ps[w][g][part * R + r][col] = __builtin_bit_cast(uint16_t, h);
+                    ps[g][part * R + r][col] = __builtin_bit_cast(uint16_t, h);
                 }
             }
         }
         __builtin_amdgcn_wave_barrier();
         // rows 4 part + r; the rows of absent parts and queries repeat others and are not used
-        const int row = R == 1 ? ((n >> 2) < PP ? (n >> 2) : 0) : ((n >> 2) < PP ? n : (n & 3));
+        const int row = R == 1 ? (PARTS == 2 ? (n >> 2) & 1 : 0) : (PARTS == 2 ? n & 7 : n & 3);
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 const int d = (ks * NG + g) * 2;
-                bf16x8 lo, hi;
+                f16x8 lo, hi;
                 kv4_v_operands(cur.v[d >> 2][d & 3], cur.v[d >> 2][(d & 3) + 1], lo, hi);
-                const u32x4 raw = *reinterpret_cast<const u32x4*>(&ps[w][g][row][ks * 32 + quad * 8]);
-                const bf16x8 pop = __builtin_bit_cast(bf16x8, raw);
+                const u32x4 raw = *reinterpret_cast<const u32x4*>(&ps[g][row][ks * 32 + quad * 8]);
+                const f16x8 pop = __builtin_bit_cast(f16x8, raw);
                 acc[2 * g] = kv4_mfma(pop, lo, acc[2 * g]);
                 acc[2 * g + 1] = kv4_mfma(pop, hi, acc[2 * g + 1]);
             }
         __builtin_amdgcn_wave_barrier();
-        if (more) cur = nxt;
+        if (more) cur.load_v(ahead, lane);
     }
 
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const float lt = wave_sum(l[r]) * (1.f / KV4_UP);
+        const float lt = wave_sum(l[r]);
         float zt[NG];
 #pragma unroll
-        for (int g = 0; g < NG; ++g) zt[g] = wave_sum(zs[r][g]) * (1.f / KV4_UP);
+        for (int g = 0; g < NG; ++g) zt[g] = wave_sum(zs[r][g]);
 #pragma unroll
         for (int c = 0; c < 2 * NG; ++c) {
-            const float v = acc[c][r];
-            float u = v + __shfl_xor(v, 16);                    // parts 0 + 1 (quads 0 and 1)
-            if (PP == 3) u += __shfl_xor(v, 32);                // quad 0: + part 2
-            u = fmaf(u, (c & 1) ? KV4_DOWN / 16.f : KV4_DOWN, zt[c >> 1]);
+            float u = acc[c][r];
+            if (PARTS == 2) u += __shfl_xor(u, 16);             // quads 0 and 1
+            u = fmaf(u, (c & 1) ? 0x1p20f : 0x1p24f, zt[c >> 1]);
             if (quad == 0) om[w][r][c * 16 + n] = u;
         }
         if (lane == 0) {
-            om[w][r][DP] = m[r];
+            om[w][r][DP] = m[r] == KV4_NONE ? -INFINITY : ref[r];
             om[w][r][DP + 1] = lt;
         }
     }
@@ -336,88 +409,94 @@ __global__ __launch_bounds__(64 * W) void kv4_few_kernel(Kv4AttnArgs a) {
 //   scores   tokens x queries: lane (quad, n) holds tokens 16 t + 4 quad + 0..3 of query n
 //   p s      is an operand as it lies (slots 0-3 from tile 2 ks, 4-7 from 2 ks + 1, the order of the V codes)
 //   context  features x queries: lane (quad, n) holds features 16 c + 4 quad + 0..3 of query n
-// The (s, z) pairs are one a token and reach the lanes through LDS.
+// Bound by vector instructions (16 scores a lane and block): what can be a product is one.  The zeros' share of a score,
+// sum_g z_tg Q_g, is a product of 8 slots (z exact in fp16, Q in two parts), sum_t p_t z_tg and sum_t p_t are rows of one
+// more product of p.  Scales and zeros are one a token and reach the lanes through LDS; a group that is NaN has a NaN
+// scale, its zero is taken as 0 so that rows that do not see the token stay clean.
 template <typename T, int NG, int W>
-__global__ __launch_bounds__(64 * W) void kv4_many_kernel(Kv4AttnArgs a) {
+__global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnArgs a) {
     constexpr bool F32 = sizeof(T) == 4;
-    constexpr int QP = F32 ? 3 : 1, PP = F32 ? 3 : 2;
+    constexpr int PARTS = F32 ? 2 : 1;
     constexpr int DP = NG * 32;
-    __shared__ __align__(16) uint32_t meta[W][2][KV4_TOK * NG];
-    __shared__ float om[W][16][DP + 4];
+    struct Token {
+        float vs[NG][KV4_TOK];              // V scales * 2^-exponent
+        uint16_t ks[NG][KV4_TOK];           // K scales
+        uint16_t vz[NG][KV4_TOK];           // V zeros in the operand's token order
+        uint2 kz[KV4_TOK];                  // K zeros, groups 0..3
+    };
+    __shared__ __align__(16) Token tk[kv4_waves(W)];
+    __shared__ float om_[kv4_waves(W) / W][W][16][DP + 4];
 
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, quad = lane >> 4;
-    const Kv4Work wk(a, 16);
-    bf16x8 qop[QP][NG];
-    float qsum[NG];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = W == 1 ? 0 : wave;
+    const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
+    const uint32_t id = W == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+    if (W == 1 && id >= a.units) return;
+    auto& om = om_[W == 1 ? wave : 0];
+    Kv4Work wk(a, 16, id);
+    wk.span(a);
     const int qi = wk.q0 + n;
     const bool have = qi < a.NQ;
     const int64_t lim = have ? (a.causal ? wk.len - a.Tq + 1 + qi % a.Tq : wk.len) : 0;
     // every row of the block sees at least this many tokens: blocks below it need no comparisons
-    const int64_t sure = a.causal ? wk.len - a.Tq + 1 : wk.len;
+    const int64_t sure = wk.q0 + 16 > a.NQ ? 0 : a.causal ? wk.len - a.Tq + 1 : wk.len;
+    Kv4Query<T, NG, PARTS> q;
     {
         const int i = have ? qi % a.Tq : 0, h = wk.hk * a.G + (have ? qi / a.Tq : 0);
-        const T* src = (const T*)a.q + wk.b * a.q_bs + h * a.q_hs + i * a.q_ts;
+        q.load((const T*)a.q + (int64_t)wk.b * a.q_bs + (int64_t)h * a.q_hs + (int64_t)i * a.q_ts, have, a.dh, quad);
+    }
+    // Q_g * 2^(up - 6) (below 2^13) in two parts: slots 0-3 and 4-7 of quad 0, against z_0..3 twice
+    f16x8 qz = {};
+    if (quad == 0) {
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            const int ch = g * 32 + quad * 8;
-            bf16x8 op[QP];
-            float sum = kv4_query<T, QP>(src + ch, have && ch < a.dh, op);
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            qsum[g] = sum * a.scale;
-#pragma unroll
-            for (int p = 0; p < QP; ++p) qop[p][g] = op[p];
+            const float y = __builtin_amdgcn_ldexpf(q.sum[g], q.up - 6);
+            qz[g] = (f16)y;
+            qz[4 + g] = (f16)(y - (float)qz[g]);
         }
     }
-    float m = -INFINITY, l = 0.f, zs[NG];
-    f32x4 acc[2 * NG];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) zs[g] = 0.f;
+    const float down = __builtin_amdgcn_ldexpf(a.scale, 24 - q.up), downz = __builtin_amdgcn_ldexpf(a.scale, 6 - q.up);
+    float m = 0.f;                               // (of no meaning while the row is fresh: it has seen no token yet)
+    bool fresh = true;
+    float vtop = 0.f;                            // the largest V scale met; scales are taken times 2^-vexp, which bounds it
+    int vexp = 0;
+    f32x4 acc[2 * NG], accz = {0.f, 0.f, 0.f, 0.f};         // accz: quad 0: sum p z_g, quad 1: sum p
 #pragma unroll
     for (int c = 0; c < 2 * NG; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const uint8_t* base = a.data + wk.bh * a.blocks * kv4_block_bytes(NG);
-    const float down = KV4_DOWN * a.scale;
+    const uint8_t* base = a.data + (int64_t)wk.bh * a.blocks * kv4_block_bytes(NG);
+    const int col = (lane & 32) | ((lane & 12) << 1) | ((lane & 16) >> 2) | ((lane & 1) << 1) | ((lane >> 1) & 1);
     const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
+    Token& my = tk[wave];
 
-    Kv4Tile<NG> cur, nxt;
-    if (wk.first + w < wk.last) cur.load(base + (wk.first + w) * kv4_block_bytes(NG), lane);
-    for (int64_t blk = wk.first + w; blk < wk.last; blk += W) {
-        const bool more = blk + W < wk.last;
-        if (more) nxt.load(base + (blk + W) * kv4_block_bytes(NG), lane);
-        const bool edge = (blk + 1) * KV4_TOK > sure;
-        const int64_t left = lim - blk * KV4_TOK, kept = wk.len - blk * KV4_TOK;
-        const int see = (int)(left > KV4_TOK ? KV4_TOK : left);      // tokens of this block that the row sees
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            meta[w][0][lane * NG + g] = lane < kept ? cur.mk[g] : 0u;
-            meta[w][1][lane * NG + g] = lane < kept ? cur.mv[g] : 0u;
-        }
-        __builtin_amdgcn_wave_barrier();
+    Kv4Tile<NG> cur;
+    auto step = [&](auto edge_c, int see, const uint32_t (&mv)[NG], const uint8_t* next) {
+        constexpr bool EDGE = decltype(edge_c)::value;
         float s[4][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             f32x4 d[NG];
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const bf16x8 kop = kv4_k_operand(cur.k[(t * NG + g) >> 2][(t * NG + g) & 3]);
-                d[g] = kv4_mfma(kop, qop[0][g], zero4);
-#pragma unroll
-                for (int p = 1; p < QP; ++p) d[g] = kv4_mfma(kop, qop[p][g], d[g]);
+                const f16x8 kop = kv4_k_operand(cur.k[(t * NG + g) >> 2][(t * NG + g) & 3]);
+                d[g] = kv4_mfma(kop, q.op[0][g], zero4);
+                if constexpr (PARTS == 2) d[g] = kv4_mfma(kop, q.op[PARTS - 1][g], d[g]);
             }
-            uint32_t mk[4 * NG];
-            __builtin_memcpy(mk, __builtin_assume_aligned(&meta[w][0][(16 * t + 4 * quad) * NG], 16), 16 * NG);
+            const uint2 z2 = my.kz[16 * t + n];
+            const u32x4 z4 = {z2.x, z2.y, z2.x, z2.y};
+            const f32x4 dz = kv4_mfma(__builtin_bit_cast(f16x8, z4), qz, zero4);
+            float dot[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float dot = 0.f, off = 0.f;
+            for (int g = 0; g < NG; ++g) {
+                uint32_t k2[2];
+                __builtin_memcpy(k2, __builtin_assume_aligned(&my.ks[g][16 * t + 4 * quad], 8), 8);
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    dot = fmaf(d[g][r], kv4_scale(mk[r * NG + g]), dot);
-                    off = fmaf(qsum[g], kv4_zero(mk[r * NG + g]), off);
-                }
-                s[t][r] = fmaf(dot, down, off);
+                for (int r = 0; r < 4; ++r) dot[r] = fmaf(d[g][r], kv4_half((k2[r >> 1] >> (16 * (r & 1))) & 0xffffu), dot[r]);
             }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[t][r] = fmaf(dot[r], down, fmaf(dz[r], downz, -m));      // relative to m
+            __builtin_amdgcn_sched_barrier(0);   // a tile at a time: all at once would take the registers of a whole wave
         }
-        if (edge) {
+        if (next) cur.load_k(next, lane);
+        if (EDGE) {
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -426,148 +505,239 @@ __global__ __launch_bounds__(64 * W) void kv4_many_kernel(Kv4AttnArgs a) {
         float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
 #pragma unroll
         for (int t = 1; t < 4; ++t) top = fmaxf(top, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
-        if (__any(top - KV4_UPLOG > m + KV4_LAZY)) {
+        float big = 0.f;                         // NaN scales are passed over: they make their own features NaN and no others
+#pragma unroll
+        for (int g = 0; g < NG; ++g) big = fmaxf(big, kv4_scale(mv[g]));
+        if (__any(top > KV4_LAZY + KV4_UP || (fresh && top > -INFINITY) || big > vtop)) {
+            vtop = fmaxf(vtop, wave_max(big));
+            const int e = vtop > 0.f ? __builtin_amdgcn_frexp_expf(vtop) : 0;
+            const float shrink = __builtin_amdgcn_ldexpf(1.f, vexp - e);
+            vexp = e;
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
-            const float mn = fmaxf(m, top - KV4_UPLOG);
-            const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            l *= f;
+            // by how much this row's reference moves: up, or wherever its first tokens are
+            const float up = !fresh ? fmaxf(top - KV4_UP, 0.f) : top > -INFINITY ? top - KV4_UP : 0.f;
+            const float f = fresh ? 1.f : __builtin_amdgcn_exp2f(-up);
+            fresh = fresh && !(top > -INFINITY);
+            m += up;
+            accz *= f;
 #pragma unroll
-            for (int g = 0; g < NG; ++g) zs[g] *= f;
+            for (int c = 0; c < 2 * NG; ++c) acc[c] *= f * shrink;
 #pragma unroll
-            for (int c = 0; c < 2 * NG; ++c) acc[c] *= f;
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[t][r] -= up;
         }
+        const float vmul = __builtin_amdgcn_ldexpf(1.f, -vexp);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const float vz = kv4_zero(mv[g]);
+            my.vs[g][lane] = kv4_scale(mv[g]) * vmul;
+            my.vz[g][col] = vz == vz ? (uint16_t)(mv[g] >> 16) : (uint16_t)0;
+        }
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const bool on = !edge || 16 * t + 4 * quad + r < see;
-                s[t][r] = on ? __builtin_amdgcn_exp2f(s[t][r] - m) : 0.f;
-                l += s[t][r];
+                s[t][r] = __builtin_amdgcn_exp2f(s[t][r]);
             }
+        // operand order of four tokens: 0 2 1 3
+        const uint32_t one2 = n == 4 ? 0x3c003c00u : 0u;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-            uint32_t mv[2][4 * NG];
+            f16x8 pop[PARTS];
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                __builtin_memcpy(mv[h], __builtin_assume_aligned(&meta[w][1][(32 * ks + 16 * h + 4 * quad) * NG], 16), 16 * NG);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float y = s[2 * ks + h][(j >> 1) | ((j & 1) << 1)];
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part) {
+                        const f16 b = (f16)y;
+                        y -= (float)b;
+                        pop[part][4 * h + j] = b;
+                    }
+                }
+            u32x4 zop = {one2, one2, one2, one2};
+            if (n < NG) zop = *reinterpret_cast<const u32x4*>(&my.vz[n < NG ? n : 0][32 * ks + 8 * quad]);
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) accz = kv4_mfma(__builtin_bit_cast(f16x8, zop), pop[part], accz);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                bf16x8 pop[PP];
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2; ++h) {
+                    const int t = 2 * ks + h;
+                    const f32x4 v4 = *reinterpret_cast<const f32x4*>(&my.vs[g][16 * t + 4 * quad]);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const int r = (j >> 1) | ((j & 1) << 1), t = 2 * ks + h;            // order 0 2 1 3
-                        const float p = s[t][r];
-                        const bool on = !edge || 16 * t + 4 * quad + r < see;
-                        float y = p * kv4_scale(mv[h][r * NG + g]);
-                        float z = p * kv4_zero(mv[h][r * NG + g]);
-                        if (edge) { y = on ? y : 0.f; z = on ? z : 0.f; }
-                        zs[g] += z;
+                        const int r = (j >> 1) | ((j & 1) << 1);
+                        float y = s[t][r] * v4[r];
+                        if (EDGE) y = 16 * t + 4 * quad + r < see ? y : 0.f;            // a scale may be NaN
 #pragma unroll
-                        for (int part = 0; part < PP; ++part) {
-                            const bf16 b = (bf16)y;
+                        for (int part = 0; part < PARTS; ++part) {
+                            const f16 b = (f16)y;
                             y -= (float)b;
                             pop[part][4 * h + j] = b;
                         }
                     }
+                }
                 const int d = (ks * NG + g) * 2;
-                bf16x8 lo, hi;
+                f16x8 lo, hi;
                 kv4_v_operands(cur.v[d >> 2][d & 3], cur.v[d >> 2][(d & 3) + 1], lo, hi);
 #pragma unroll
-                for (int part = 0; part < PP; ++part) {
+                for (int part = 0; part < PARTS; ++part) {
                     acc[2 * g] = kv4_mfma(lo, pop[part], acc[2 * g]);
                     acc[2 * g + 1] = kv4_mfma(hi, pop[part], acc[2 * g + 1]);
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
+    };
+
+    const uint8_t* ahead = base + (int64_t)(wk.first + w) * kv4_block_bytes(NG);
+    if (wk.first + w < wk.last) {
+        cur.load_k(ahead, lane);
+        cur.load_v(ahead, lane);
+    }
+    for (int blk = wk.first + w; blk < wk.last; blk += W) {
+        const bool more = blk + W < wk.last;
+        ahead += W * kv4_block_bytes(NG);
+        const int64_t at = (int64_t)blk * KV4_TOK;
+        const bool kept = lane < wk.len - at;
+        uint32_t z[4] = {0u, 0u, 0u, 0u}, mv[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {           // past the sentence's end the cache may hold anything
+            const uint32_t mk = kept ? cur.mk[g] : 0u;
+            const float kz = kv4_zero(mk);
+            mv[g] = kept ? cur.mv[g] : 0u;
+            z[g] = kz == kz ? mk >> 16 : 0u;
+            my.ks[g][lane] = (uint16_t)mk;
+        }
+        my.kz[lane] = make_uint2(z[0] | (z[1] << 16), z[2] | (z[3] << 16));
         __builtin_amdgcn_wave_barrier();
-        if (more) cur = nxt;
+        if ((int64_t)(blk + 1) * KV4_TOK > sure) {
+            const int64_t left = lim - at;
+            step(std::true_type{}, (int)(left > KV4_TOK ? KV4_TOK : left), mv, more ? ahead : nullptr);
+        } else {
+            step(std::false_type{}, KV4_TOK, mv, more ? ahead : nullptr);
+        }
+        __builtin_amdgcn_wave_barrier();
+        if (more) cur.load_v(ahead, lane);
     }
 
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    const float unit = __builtin_amdgcn_ldexpf(1.f, 24 + vexp);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-        float z = zs[g];
-        z += __shfl_xor(z, 16);
-        z += __shfl_xor(z, 32);
-        z *= 1.f / KV4_UP;
+        const float z = __shfl(accz[g], n);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                om[w][n][g * 32 + h * 16 + quad * 4 + r] = fmaf(acc[2 * g + h][r], h ? KV4_DOWN / 16.f : KV4_DOWN, z);
+                om[w][n][g * 32 + h * 16 + quad * 4 + r] = fmaf(acc[2 * g + h][r], h ? unit / 16.f : unit, z);
     }
-    if (quad == 0) {
-        om[w][n][DP] = m;
-        om[w][n][DP + 1] = l * (1.f / KV4_UP);
+    if (quad == 1) {
+        om[w][n][DP] = fresh ? -INFINITY : m;
+        om[w][n][DP + 1] = accz[0];
     }
     if (W > 1) __syncthreads();
     else __builtin_amdgcn_wave_barrier();
     kv4_finish<T, W, 16, DP>(a, wk, om);
 }
 
-// joins the splits of a query row: one wave a row
+// Joins the splits of a query row: the factors once for all, then every wave a quarter of the splits, two features a lane.
 template <typename T>
-__global__ __launch_bounds__(64) void kv4_join_kernel(Kv4AttnArgs a) {
+__global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a) {
+    __shared__ float fac[KV4_MAX_SPLITS], red[4][KV4_MAX_DH], sums[4];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t row = blockIdx.x;
-    const float* ml = a.part + a.rows * a.splits * a.dh + row * a.splits * 2;
-    float top = -INFINITY;
-    for (int s = threadIdx.x; s < a.splits; s += 64) top = fmaxf(top, ml[2 * s]);
-    top = wave_max(top);
-    float sum = 0.f, o0 = 0.f, o1 = 0.f;
-    const int c0 = threadIdx.x, c1 = c0 + 64;
+    const float2* ml = reinterpret_cast<const float2*>(a.part + a.rows * a.splits * a.dh) + row * a.splits;
     const float* o = a.part + row * a.splits * a.dh;
-    for (int s = 0; s < a.splits; ++s) {
-        const float m = ml[2 * s], l = ml[2 * s + 1];
-        const float f = m == -INFINITY && l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - top);
-        sum = fmaf(f, l, sum);
-        if (c0 < a.dh) o0 = fmaf(f, o[(int64_t)s * a.dh + c0], o0);
-        if (c1 < a.dh) o1 = fmaf(f, o[(int64_t)s * a.dh + c1], o1);
+    float top = -INFINITY;
+    for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, ml[s].x);      // every wave for itself
+    top = wave_max(top);
+    float sum = 0.f;
+    for (int s = threadIdx.x; s < a.splits; s += 256) {
+        const float2 x = ml[s];
+        const float f = x.x == -INFINITY && x.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x.x - top);
+        fac[s] = f;
+        sum = fmaf(f, x.y, sum);
     }
+    sum = wave_sum(sum);
+    if (lane == 0) sums[w] = sum;
+    __syncthreads();
+    sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    float o0 = 0.f, o1 = 0.f;
+    const int c = 2 * lane;
+    if (c < a.dh) {
+#pragma unroll 4
+        for (int s = w; s < a.splits; s += 4) {
+            const float2 x = *reinterpret_cast<const float2*>(o + (int64_t)s * a.dh + c);
+            o0 = fmaf(fac[s], x.x, o0);
+            o1 = fmaf(fac[s], x.y, o1);
+        }
+        red[w][c] = o0;
+        red[w][c + 1] = o1;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x >= a.dh) return;
+    const float v = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
     const int64_t bh = row / a.NQ;
     const int qi = (int)(row % a.NQ), i = qi % a.Tq;
     const int64_t b = bh / a.Hkv, h = (bh % a.Hkv) * a.G + qi / a.Tq;
-    T* dst = (T*)a.out + b * a.o_bs + h * a.o_hs + i * a.o_ts;
-    if (c0 < a.dh) dst[c0] = from_f<T>(sum == 0.f ? 0.f : o0 / sum);
-    if (c1 < a.dh) dst[c1] = from_f<T>(sum == 0.f ? 0.f : o1 / sum);
+    ((T*)a.out)[b * a.o_bs + h * a.o_hs + i * a.o_ts + threadIdx.x] = from_f<T>(sum == 0.f ? 0.f : v / sum);
 }
 
 struct Kv4Shape { int rows, W, splits; int64_t units; };
 
-// How a call is cut: `longest` bounds the lengths (the capacity where the caller knows no better).
-static Kv4Shape kv4_shape(int64_t B, int Hkv, int NQ, int64_t longest) {
+// How a call is cut: `longest` bounds the lengths (the capacity where the caller knows no better), nb is that in blocks of
+// 64 tokens, units the (sentence, key/value head, query rows) triples.  Measured on graph replays, us:
+//   a wave each (W = 1) where units fill the chip: 4096 units of 140 tokens 12.5 against 18.7 with four waves; 2048 units
+//     of 1200 tokens 39.8 against 41.2, of more it evens out
+//   eight waves where units are few: 8 units of 1200 tokens 5.5 against 6.7 with four; 256 units of 5000 tokens 20 against
+//     25; but 512 units of 300 tokens 6.1 against 5.7, and many-row kernels on 512 units 10.9 against 8.0
+//   splits, whose joining costs a second launch (3 us), where a unit's waves would go round more than four times and the
+//     chip has room: 8 units of 5000 tokens 7.2 against 11.3, 64 units (4 rows) of 8190 tokens 22 against 47; with 256
+//     units of 10000 tokens 42 against 38 unsplit.  128 units of 0 .. 32768 tokens: 8 splits 36, 2 splits 47.
+static Kv4Shape kv4_shape(int64_t B, int Hkv, int NQ, int ng, int64_t longest) {
     Kv4Shape s;
     s.rows = NQ == 1 ? 1 : NQ <= 4 ? 4 : 16;
     s.units = B * Hkv * ((NQ + s.rows - 1) / s.rows);
     const int64_t nb = (longest + KV4_TOK - 1) / KV4_TOK;
-    s.W = nb <= 1 || s.units >= 4096 ? 1 : 4;
-    const int64_t want = 4096 / (s.units * s.W), most = (nb + s.W - 1) / s.W;
+    const bool crowd = s.units >= 2048 && nb <= 16;
+    const bool eight = s.rows != 4 && nb > 4 && (s.units <= 256 || (s.rows == 1 && nb >= 24));
+    s.W = nb <= 1 || crowd ? 1 : eight ? 8 : 4;
+    int64_t want = 1;
+    if (s.rows == 1 && nb >= 36 && s.units <= 128) {
+        const int64_t room = 1024 / s.units, use = nb / (8 * (1 + s.units / 64));
+        want = room < use ? room : use;
+    }
+    if (s.rows == 4 && nb >= 16 + s.units / 16) want = (ng <= 2 ? 512 : 256) / s.units;
+    if (s.rows == 16 && nb >= 20) want = 256 / s.units;
+    const int64_t most = (nb + s.W - 1) / s.W;
     s.splits = (int)(want < 1 ? 1 : (want > most ? most : want));
-    if (s.splits > 512) s.splits = 512;
+    if (s.splits > KV4_MAX_SPLITS) s.splits = KV4_MAX_SPLITS;
     return s;
 }
 
 template <typename T, int NG, int W>
 static void kv4_launch(const Kv4AttnArgs& a, const Kv4Shape& s, hipStream_t st) {
-    const unsigned grid = (unsigned)(s.units * s.splits);
-    if (s.rows == 1) kv4_few_kernel<T, NG, 1, W><<<grid, 64 * W, 0, st>>>(a);
-    else if (s.rows == 4) kv4_few_kernel<T, NG, 4, W><<<grid, 64 * W, 0, st>>>(a);
-    else kv4_many_kernel<T, NG, W><<<grid, 64 * W, 0, st>>>(a);
+    const unsigned grid = W == 1 ? (a.units + 3) / 4 : a.units, threads = 64 * kv4_waves(W);
+    if (s.rows == 1) kv4_few_kernel<T, NG, 1, W><<<grid, threads, 0, st>>>(a);
+    else if (s.rows == 16) kv4_many_kernel<T, NG, W><<<grid, threads, 0, st>>>(a);
+    else if constexpr (W != 8) kv4_few_kernel<T, NG, 4, W><<<grid, threads, 0, st>>>(a);
 }
 template <typename T>
 static void kv4_dispatch(const Kv4AttnArgs& a, const Kv4Shape& s, int ng, hipStream_t st) {
 #define MSSR_KV4_A(NG)                                \
     case NG:                                          \
         if (s.W == 1) kv4_launch<T, NG, 1>(a, s, st); \
-        else kv4_launch<T, NG, 4>(a, s, st);          \
+        else if (s.W == 4) kv4_launch<T, NG, 4>(a, s, st); \
+        else kv4_launch<T, NG, 8>(a, s, st);          \
         break;
     switch (ng) { MSSR_KV4_A(1) MSSR_KV4_A(2) MSSR_KV4_A(3) MSSR_KV4_A(4) }
 #undef MSSR_KV4_A
-    if (a.splits > 1) kv4_join_kernel<T><<<(unsigned)a.rows, 64, 0, st>>>(a);
+    if (a.splits > 1) kv4_join_kernel<T><<<(unsigned)a.rows, 256, 0, st>>>(a);
 }
 
 }  // namespace mssr
@@ -582,7 +752,7 @@ extern "C" int64_t mssr_kv4_attention_scratch(const mssr_kv4_cache* c, int64_t T
     if (!c || c->B < 1 || c->H < 1 || H < c->H || H % c->H || Tq < 1 || c->capacity < 1 || !valid_dtype(dtype)) return -1;
     if (Tq > INT32_MAX / (H / c->H)) return -1;
     const int NQ = (int)(H / c->H * Tq);
-    const Kv4Shape s = kv4_shape(c->B, c->H, NQ, kv4_longest(c, longest));
+    const Kv4Shape s = kv4_shape(c->B, c->H, NQ, kv4_groups(c->dh), kv4_longest(c, longest));
     return s.splits > 1 ? c->B * c->H * NQ * s.splits * (c->dh + 2) * (int64_t)sizeof(float) : 0;
 }
 
@@ -594,6 +764,7 @@ extern "C" int mssr_kv4_attention(const mssr_kv4_cache* c, const void* q, int64_
     MSSR_REQUIRE(mssr_kv4_bytes(c->B, c->H, c->capacity, c->dh) > 0 && aligned(c->data, 16),
                  "kv4_attention: cache of %lld x %d heads x %lld tokens x %d features (multiples of 8 up to %d)",
                  (long long)c->B, c->H, (long long)c->capacity, c->dh, KV4_MAX_DH);
+    MSSR_REQUIRE(c->capacity <= (int64_t)KV4_TOK * INT32_MAX, "kv4_attention: %lld tokens a sentence", (long long)c->capacity);
     MSSR_REQUIRE(valid_dtype(dtype), "kv4_attention: dtype %d", dtype);
     MSSR_REQUIRE(Tq >= 0 && H >= c->H && H % c->H == 0, "kv4_attention: %d query heads on %d, %lld rows", H, c->H, (long long)Tq);
     MSSR_REQUIRE(lengths || (length0 >= 0 && length0 <= c->capacity), "kv4_attention: length %lld of a cache of %lld",
@@ -601,7 +772,7 @@ extern "C" int mssr_kv4_attention(const mssr_kv4_cache* c, const void* q, int64_
     if (Tq == 0) return MSSR_OK;
     MSSR_REQUIRE(Tq <= (INT32_MAX >> 8) / (H / c->H), "kv4_attention: %lld query rows", (long long)Tq);
     const int NQ = (int)(H / c->H * Tq);
-    const Kv4Shape s = kv4_shape(c->B, c->H, NQ, kv4_longest(c, longest));
+    const Kv4Shape s = kv4_shape(c->B, c->H, NQ, kv4_groups(c->dh), kv4_longest(c, longest));
     const int64_t rows = c->B * c->H * NQ;
     MSSR_REQUIRE(s.units <= KV4_MAX_GRID / s.splits && rows <= KV4_MAX_GRID, "kv4_attention: %lld query rows in one call",
                  (long long)rows);
@@ -609,7 +780,7 @@ extern "C" int mssr_kv4_attention(const mssr_kv4_cache* c, const void* q, int64_
                  "kv4_attention: scratch of %lld bytes is too small", (long long)scratch_bytes);
     Kv4AttnArgs a{(const uint8_t*)c->data, (c->capacity + KV4_TOK - 1) / KV4_TOK, c->capacity, q, out, q_bs, q_hs, q_ts,
                   o_bs, o_hs, o_ts, c->H, H / c->H, (int)Tq, c->dh, causal ? 1 : 0, NQ, s.splits,
-                  {lengths, lengths_are_64, length0}, scale * 1.4426950408889634f, (float*)scratch, rows};
+                  {lengths, lengths_are_64, length0}, scale * 1.4426950408889634f, (float*)scratch, rows, (uint32_t)(s.units * s.splits)};
     if (dtype == MSSR_F32) kv4_dispatch<float>(a, s, kv4_groups(c->dh), (hipStream_t)stream);
     else kv4_dispatch<bf16>(a, s, kv4_groups(c->dh), (hipStream_t)stream);
     MSSR_LAUNCH_OK("kv4_attention");

@@ -37,16 +37,19 @@ def values(x):
 
 
 def attend(q, k, v, lengths, scale, causal):
-    """-> (context, bound): the formula in 64 bits over the values k, v stand for, and how far fp32 arithmetic on the codes
-    may be from it before the result is rounded.  Per row, with u = 2^-24 the fp32 half step:
-      a score's products add up in fp32 (at most 34 roundings a group, a few for scales and zeros, one of scale * log2 e):
-        |ds| <= 44 u sum_c |q_c| (|z| + 15 s + |k|)  (bounded by 3 max|k| for the bracket's terms), exp2 adds 2 u;
+    """-> (context, bound): the formula in 64 bits over the values k, v stand for, and how far the kernels' arithmetic on
+    the codes may be from it before the result is rounded.  Per row, with u = 2^-24 the fp32 half step:
+      a score: q is one fp16 part (bf16: exact but for 2^-39 of the row's largest element) or two (fp32: 2^-22 = 4 u each);
+        its products add up in fp32 (at most 34 roundings a group, a few for scales and zeros, one of scale * log2 e):
+        |ds| <= 48 u sum_c |q_c| (|z| + 15 s + |k|)  (bounded by 3 max|k| for the bracket's terms), exp2 adds 2 u;
       so p is off by a factor 1 +- (|ds| + 4 u), and the quotient by twice that of max |v|;
-      p s as bf16 parts: 2^-17 (two parts) or 2^-24 (three); sums over n tokens: n / 8 + 40 roundings (a matrix product
-      adds 32 terms at a time, then blocks, waves and splits are joined)."""
+      p s is one fp16 part (bf16: 2^-11) or two (fp32: 2^-22), and where it is below 2^-21 of the largest scale at most
+        2^-32 of that scale: m tokens * 15 codes of it, 15 * scale <= 2 max |v|;
+      sums over m tokens: m / 8 + 40 roundings (a matrix product adds 32 terms at a time, then blocks, waves and splits
+        are joined)."""
     B, H, T, dh = q.shape
     G = H // k.shape[1]
-    two = q.dtype == torch.bfloat16
+    bf16 = q.dtype == torch.bfloat16
     out = torch.zeros(B, H, T, dh, dtype=torch.float64, device=q.device)
     bound = torch.zeros(B, H, T, 1, dtype=torch.float64, device=q.device)
     u = 2.0 ** -24
@@ -60,8 +63,8 @@ def attend(q, k, v, lengths, scale, causal):
                     continue
                 qq = q[b, h, i].double()
                 out[b, h, i] = torch.softmax(scale * (kk[:m] @ qq), 0) @ vv[:m]
-                ds = 44 * u * abs(scale) * float(qq.abs().sum()) * 3 * float(kk[:m].abs().max())
-                rel = 2 * (ds + 4 * u) + (2.0 ** -17 if two else u) + (m / 8 + 40) * u
+                ds = 48 * u * abs(scale) * float(qq.abs().sum()) * 3 * float(kk[:m].abs().max())
+                rel = 2 * (ds + 4 * u) + (2.0 ** -11 if bf16 else 4 * u) + m * 2.0 ** -32 + (m / 8 + 40) * u
                 # zeros and codes are summed apart: up to |z| + 15 s <= 3 max |v| a term
                 bound[b, h, i] = rel * 3 * float(vv[:m].abs().max())
     return out, bound
