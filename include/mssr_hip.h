@@ -696,7 +696,7 @@ typedef struct {
     void* scratch;                /* mssr_token_control_scratch() bytes where ids is given */
     int64_t scratch_bytes;
 } mssr_token_control_desc;
-int64_t mssr_token_control_scratch(int64_t B, int64_t V);
+int64_t mssr_token_control_scratch(int64_t B, int64_t V, int64_t T);
 int mssr_token_control(const mssr_token_control_desc* desc, void* stream);
 
 #ifdef __cplusplus

@@ -190,7 +190,7 @@ SIGNATURES = {
     "mssr_kv4_attention_scratch": ([POINTER(Kv4Cache), _L, _I, _L, _I], c_int64),
     "mssr_kv4_attention": ([POINTER(Kv4Cache), _P, _L, _L, _L, _P, _L, _L, _L, _I, _L, _P, _L, _I, _L, _F, _I, _P, _L, _I, _P],
                            c_int),
-    "mssr_token_control_scratch": ([_L, _L], c_int64),
+    "mssr_token_control_scratch": ([_L, _L, _L], c_int64),
     "mssr_token_control": ([POINTER(TokenControlDesc), _P], c_int),
     "mssr_debug_stamps": ([_P], None),
     "mssr_ctx_kv_grad": ([_P, _P, _L, _P, _L, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P], c_int),

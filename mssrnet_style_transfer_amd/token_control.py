@@ -149,7 +149,7 @@ def _call(who, logits, control, history, lengths, prompt_lengths, out, ids, empt
     lib, ptr, ws, need = L.load(), L.ptr, None, 0
     if ids is not None:
         bits |= 16 * int(ids.dtype is torch.int64)
-        need = lib.mssr_token_control_scratch(B, V)
+        need = lib.mssr_token_control_scratch(B, V, T)
         if need > 0:                             # a call's own: streams and captured graphs share none
             ws = torch.empty(need, dtype=torch.uint8, device=dev)
     d = L.TokenControlDesc(logits.data_ptr(), ptr(out), B, V, logits.stride(0) if B > 1 else V,

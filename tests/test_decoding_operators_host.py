@@ -85,8 +85,9 @@ def test_token_control_refusals():
     assert L.load().mssr_token_control(None, None) == 1
     assert control(B=0, logits=None) == 0
     lib = L.load()
-    assert lib.mssr_token_control_scratch(0, 5) == -1 and lib.mssr_token_control_scratch(1, 0) == -1
-    assert lib.mssr_token_control_scratch(1, 20) == 0 and lib.mssr_token_control_scratch(1, 100000) > 0
+    for B, V, T in ((0, 5, 0), (1, 0, 0), (1, 5, -1), (1, 5, 1 << 30), (1, 1 << 31, 0)):
+        assert lib.mssr_token_control_scratch(B, V, T) == -1
+    assert lib.mssr_token_control_scratch(1, 20, 0) == 0 and lib.mssr_token_control_scratch(1, 100000, 0) > 0
 
 
 def test_pack_allowed():
