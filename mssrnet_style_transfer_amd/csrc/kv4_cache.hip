@@ -42,24 +42,26 @@ __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
 
 // The group's codes of this lane's 8 features (one byte each, features 0-3 in c0, 4-7 in c1) and its (s, z) word.
 // `live`: the lane holds features (a head's last group may have fewer than 32).  All four lanes of a group call it.
-__device__ __forceinline__ void kv4_quantise(float (&x)[8], bool live, uint32_t& c0, uint32_t& c1, uint32_t& meta) {
+// Bound by vector instructions as soon as memory is not waited for, hence: minima and maxima three at a time, NaN two at a
+// time, infinities by the extremes, no clamp of the elements (codes are clamped, and x beyond the clamped extremes has the
+// extreme's code), conversion and packing in one instruction.
+__device__ __forceinline__ void kv4_quantise(const float (&x)[8], bool live, uint32_t& c0, uint32_t& c1, uint32_t& meta) {
 #pragma clang fp contract(off)
-    float lo = INFINITY, hi = -INFINITY;
-    uint32_t bad = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        bad |= (__builtin_bit_cast(uint32_t, x[i]) & 0x7f800000u) == 0x7f800000u ? 1u : 0u;
-        x[i] = fminf(fmaxf(x[i], -65504.f), 65504.f);
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
-    }
-    if (!live) { lo = INFINITY; hi = -INFINITY; bad = 0; }
+    float lo = fminf(fminf(fminf(fminf(x[0], x[1]), x[2]), fminf(fminf(x[3], x[4]), x[5])), fminf(x[6], x[7]));
+    float hi = fmaxf(fmaxf(fmaxf(fmaxf(x[0], x[1]), x[2]), fmaxf(fmaxf(x[3], x[4]), x[5])), fmaxf(x[6], x[7]));
+    bool nan = __builtin_isunordered(x[0], x[1]) | __builtin_isunordered(x[2], x[3]) | __builtin_isunordered(x[4], x[5]) |
+               __builtin_isunordered(x[6], x[7]);
+    lo = live ? (nan ? -INFINITY : lo) : INFINITY;
+    hi = live ? hi : -INFINITY;
     lo = fminf(lo, dpp_mov<0xB1>(lo));
     hi = fmaxf(hi, dpp_mov<0xB1>(hi));
-    bad |= dpp_u32<0xB1>(bad);
     lo = fminf(lo, dpp_mov<0x4E>(lo));
     hi = fmaxf(hi, dpp_mov<0x4E>(hi));
-    bad |= dpp_u32<0x4E>(bad);
+    const bool bad = lo == -INFINITY || hi == INFINITY;
+    lo = fmaxf(lo, -65504.f);
+    hi = fminf(hi, 65504.f);
+    lo = fminf(lo, 65504.f);
+    hi = fmaxf(hi, -65504.f);
     float step = (hi - lo) * (1.0f / 15.0f);
     // The definition rounds this product to fp32, then to fp16.  Left alone, the compiler takes both in one mixed-precision
     // instruction with a single rounding: another scale in one of some 8000 groups.
@@ -67,25 +69,25 @@ __device__ __forceinline__ void kv4_quantise(float (&x)[8], bool live, uint32_t&
     const f16 s = (f16)step;
     const f16 z = (f16)lo;
     const float sf = (float)s, zf = (float)z;
-    const float inv = sf > 0.f ? 1.0f / sf : 0.f;
+    // 1 / s, correctly rounded: one Newton step from the hardware's estimate, checked for every positive fp16 number
+    const float r0 = __builtin_amdgcn_rcpf(sf);
+    const float inv = sf > 0.f ? __builtin_fmaf(__builtin_fmaf(-sf, r0, 1.f), r0, r0) : 0.f;
     c0 = c1 = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float q = fminf(fmaxf(rintf((x[i] - zf) * inv), 0.f), 15.f);
-        const uint32_t c = live ? (uint32_t)q : 0u;
-        if (i < 4) c0 |= c << (8 * i);
-        else c1 |= c << (8 * (i - 4));
+        const float q = __builtin_rintf(__builtin_amdgcn_fmed3f((x[i] - zf) * inv, 0.f, 15.f));
+        if (i < 4) c0 = __builtin_amdgcn_cvt_pk_u8_f32(q, i, c0);
+        else c1 = __builtin_amdgcn_cvt_pk_u8_f32(q, i - 4, c1);
     }
-    if (bad) c0 = c1 = 0;
+    if (!live || bad) c0 = c1 = 0;
     meta = bad ? 0x7e007e00u
                : (uint32_t)__builtin_bit_cast(uint16_t, s) | ((uint32_t)__builtin_bit_cast(uint16_t, z) << 16);
 }
 
 // K dword of the lane: feature 2 r in nibble r, feature 2 r + 1 in nibble r + 4
 __device__ __forceinline__ uint32_t kv4_pack_k(uint32_t c0, uint32_t c1) {
-    const uint32_t even = (c0 & 0xfu) | ((c0 >> 12) & 0xf0u) | ((c1 & 0xfu) << 8) | ((c1 >> 4) & 0xf000u);
-    const uint32_t odd = ((c0 >> 8) & 0xfu) | ((c0 >> 20) & 0xf0u) | (c1 & 0xf00u) | ((c1 >> 12) & 0xf000u);
-    return even | (odd << 16);
+    const uint32_t t0 = c0 | (c0 >> 12), t1 = c1 | (c1 >> 12);       // bytes 0, 1: features (0, 2), (1, 3); (4, 6), (5, 7)
+    return __builtin_amdgcn_perm(t1, t0, 0x05010400u);
 }
 
 // This lane's four V bytes (n0 .. n0 + 3): the low nibbles come from the group's lanes 0 / 1, the high ones from 2 / 3.
@@ -146,13 +148,15 @@ __global__ __launch_bounds__(256) void kv4_write_tokens_kernel(Kv4WriteArgs a) {
 }
 
 // One cache block of one (sentence, head): its image is put together in LDS and leaves in 16-byte stores where the call
-// covers the whole block, in the dwords and bytes of the covered tokens where it does not.
+// covers the whole block, in the dwords and bytes of the covered tokens where it does not.  A thread has 8 features of four
+// consecutive tokens, so that the V codes, a byte a token, are dwords before they reach LDS.
 template <typename T, int NG>
-__global__ __launch_bounds__(256) void kv4_write_blocks_kernel(Kv4WriteArgs a, uint32_t span) {
+__global__ __launch_bounds__(64 * NG) void kv4_write_blocks_kernel(Kv4WriteArgs a, uint32_t span) {
+    constexpr int THREADS = 64 * NG;
     __shared__ __align__(16) uint8_t img[NG * 2560];
     const uint32_t bh = blockIdx.x / span, j = blockIdx.x % span;
-    const int64_t b = bh / a.c.H;
-    const int h = bh % a.c.H;
+    const int64_t b = bh / (uint32_t)a.c.H;
+    const int h = bh % (uint32_t)a.c.H;
     const int64_t start = a.start.at(b);
     int64_t cnt = a.counts.p ? a.counts.at(b) : a.T;
     cnt = cnt < 0 ? 0 : (cnt > a.T ? a.T : cnt);
@@ -162,44 +166,52 @@ __global__ __launch_bounds__(256) void kv4_write_blocks_kernel(Kv4WriteArgs a, u
     const int64_t blk = (p0 >> 6) + j, base = blk << 6;
     if (p1 <= p0 || base >= p1) return;
     const int t0 = (int)(p0 > base ? p0 - base : 0), t1 = (int)(p1 - base < KV4_TOK ? p1 - base : KV4_TOK);
-    const T* kp = (const T*)a.k + b * a.k_bs + h * a.k_hs + (base - start) * a.k_ts;
-    const T* vp = (const T*)a.v + b * a.v_bs + h * a.v_hs + (base - start) * a.v_ts;
-    float xk[NG][8], xv[NG][8];
+    const int quad = threadIdx.x & 3, g = (threadIdx.x >> 2) % NG, tok = (threadIdx.x >> 2) / NG * 4;
+    const int ch = g * 32 + quad * 8;
+    const bool live = ch < a.c.dh;
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-        const int item = i * 256 + threadIdx.x, quad = item & 3, g = (item >> 2) % NG, tok = (item >> 2) / NG;
-        const int ch = g * 32 + quad * 8;
+    for (int which = 0; which < 2; ++which) {
+        const int64_t ts = which ? a.v_ts : a.k_ts;
+        const T* src = (which ? (const T*)a.v + b * a.v_bs + h * a.v_hs : (const T*)a.k + b * a.k_bs + h * a.k_hs) +
+                       (base - start) * ts + ch;
+        float x[4][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) xk[i][e] = xv[i][e] = 0.f;
-        if (tok >= t0 && tok < t1 && ch < a.c.dh) {
-            Ld8<T>::load(kp + tok * a.k_ts + ch, xk[i]);
-            Ld8<T>::load(vp + tok * a.v_ts + ch, xv[i]);
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[e][i] = 0.f;
+            if (live && tok + e >= t0 && tok + e < t1) Ld8<T>::load(src + (tok + e) * ts, x[e]);
         }
-    }
+        uint32_t m[4], vb[4];
+        int n0 = 0;
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-        const int item = i * 256 + threadIdx.x, quad = item & 3, g = (item >> 2) % NG, tok = (item >> 2) / NG;
-        const bool live = g * 32 + quad * 8 < a.c.dh;
-        uint32_t c0, c1, m;
-        kv4_quantise(xk[i], live, c0, c1, m);
-        *reinterpret_cast<uint32_t*>(img + kv4_k_off(NG, tok, g, quad)) = kv4_pack_k(c0, c1);
-        if (quad == 0) *reinterpret_cast<uint32_t*>(img + kv4_kmeta_off(NG, tok, g)) = m;
-        kv4_quantise(xv[i], live, c0, c1, m);
-        int n0;
-        const uint32_t vb = kv4_pack_v(c0, c1, quad, n0);
-        uint8_t* q = img + kv4_v_off(NG, tok, g, n0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q[16 * e] = (uint8_t)(vb >> (8 * e));
-        if (quad == 1) *reinterpret_cast<uint32_t*>(img + kv4_vmeta_off(NG, tok, g)) = m;
+        for (int e = 0; e < 4; ++e) {
+            uint32_t c0, c1;
+            kv4_quantise(x[e], live, c0, c1, m[e]);
+            if (which) vb[e] = kv4_pack_v(c0, c1, quad, n0);
+            else *reinterpret_cast<uint32_t*>(img + kv4_k_off(NG, tok + e, g, quad)) = kv4_pack_k(c0, c1);
+        }
+        if (which) {                             // four tokens x four bytes, turned over
+            const uint32_t a01 = __builtin_amdgcn_perm(vb[1], vb[0], 0x05010400u), b01 = __builtin_amdgcn_perm(vb[1], vb[0], 0x07030602u);
+            const uint32_t a23 = __builtin_amdgcn_perm(vb[3], vb[2], 0x05010400u), b23 = __builtin_amdgcn_perm(vb[3], vb[2], 0x07030602u);
+            uint32_t* q = reinterpret_cast<uint32_t*>(img + kv4_v_off(NG, tok, g, n0));
+            q[0] = __builtin_amdgcn_perm(a23, a01, 0x05040100u);
+            q[4] = __builtin_amdgcn_perm(a23, a01, 0x07060302u);
+            q[8] = __builtin_amdgcn_perm(b23, b01, 0x05040100u);
+            q[12] = __builtin_amdgcn_perm(b23, b01, 0x07060302u);
+        }
+        // the group's four lanes have the same four pairs; each stores one token's
+        const uint32_t lo = quad & 1 ? m[1] : m[0], hi = quad & 1 ? m[3] : m[2];
+        *reinterpret_cast<uint32_t*>(img + (which ? kv4_vmeta_off(NG, tok + quad, g) : kv4_kmeta_off(NG, tok + quad, g))) =
+            quad & 2 ? hi : lo;
     }
     __syncthreads();
     uint8_t* dst = a.c.data + ((int64_t)bh * a.c.blocks + blk) * kv4_block_bytes(NG);
     if (t0 == 0 && t1 == KV4_TOK) {
-        for (int i = threadIdx.x; i < NG * 160; i += 256)
+        for (int i = threadIdx.x; i < NG * 160; i += THREADS)
             reinterpret_cast<u32x4*>(dst)[i] = reinterpret_cast<const u32x4*>(img)[i];
         return;
     }
-    for (int i = threadIdx.x; i < NG * 640; i += 256) {
+    for (int i = threadIdx.x; i < NG * 640; i += THREADS) {
         int lo, n = 1;                                  // tokens [lo, lo + n) of this dword
         if (i < NG * 256) {                             // K codes: one token
             const int d = (i >> 8) * 4 + (i & 3);
@@ -363,8 +375,8 @@ extern "C" int mssr_kv4_write(const mssr_kv4_cache* c, const void* k, int64_t k_
         const unsigned grid = (unsigned)(bh * span);
 #define MSSR_KV4_W(NG)                                                                                   \
     case NG:                                                                                             \
-        if (dtype == MSSR_F32) kv4_write_blocks_kernel<float, NG><<<grid, 256, 0, s>>>(a, (uint32_t)span); \
-        else kv4_write_blocks_kernel<bf16, NG><<<grid, 256, 0, s>>>(a, (uint32_t)span);                  \
+        if (dtype == MSSR_F32) kv4_write_blocks_kernel<float, NG><<<grid, 64 * NG, 0, s>>>(a, (uint32_t)span); \
+        else kv4_write_blocks_kernel<bf16, NG><<<grid, 64 * NG, 0, s>>>(a, (uint32_t)span);                  \
         break;
         switch (ng) { MSSR_KV4_W(1) MSSR_KV4_W(2) MSSR_KV4_W(3) MSSR_KV4_W(4) }
 #undef MSSR_KV4_W
