@@ -6,13 +6,18 @@
 // so the matrix instructions take the CODES as they lie and the scales touch only scores and probabilities: one number
 // a token instead of 32.  A code needs no conversion: the bit pattern of an integer c < 1024 read as fp16 is the number
 // c * 2^-24 (subnormals, which the matrix cores keep), so `x & 0x000f000f` IS an operand pair and `x & 0x00f000f0` one
-// that is 16 times as large.  8 codes take 5 vector instructions.
+// that is 16 times as large.  8 codes take 5 vector instructions.  (The matrix cores align a subnormal's bits as if its
+// leading one stood in place: with codes in the lowest four of ten bits, products lose what is below 2^-21 of the largest.
+// bf16 calls do not see it; fp32 ones take all codes 16 times as large, 2^-26, for two shifts more.)
 //
 // What meets the codes is fp16 too (11 bits), as parts whose products add up in fp32: one part for bf16 calls (exact for
 // q; 2^-11 of p s, averaged over tokens, where the result keeps 2^-8), two for fp32 ones (2^-22).  Powers of two keep
 // them in fp16's range: a query row is scaled to a largest element in [2^13, 2^14); p s is taken relative to the largest
 // V scale met so far (rounded up to a power of two; when it grows, the sums shrink), with p up to 2^8 (below) and 7 bits
 // on top, so that what is 2^-21 of the largest still has all its bits and the rest is off by at most 2^-32 of it.
+//
+// A product's sums are cut, not rounded, where they meet an accumulator that has outgrown them by more than 24 bits less
+// their own; fp32 calls therefore start every block of 64 tokens from zero and add it up by rounding additions.
 //
 // A wave takes 64 tokens at a time; the running maximum moves only when a score passes it by more than 8 (then every
 // sum is rescaled), so that a block of tokens costs one comparison and no cross-lane reduction.  The W waves of a block
@@ -41,28 +46,42 @@ struct Kv4AttnArgs {
 constexpr float KV4_LAZY = 8.f;          // log2 of how far a probability may pass 1 before a rescale
 constexpr float KV4_UP = 7.f;            // log2 of what probabilities are held times
 constexpr float KV4_NONE = -3e38f;       // the reference of a row that has seen no token: 2^(-inf - KV4_NONE) is 0
+constexpr int KV4_SETTLE = 16;           // blocks between two settlings of fp32 sums (kv4_few_kernel)
 constexpr int KV4_MAX_SPLITS = 512;
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-// 8 codes of a K dword -> operand whose elements 2 r, 2 r + 1 are features 2 r, 2 r + 1 (r odd: times 16)
+// 8 codes of a K dword -> operand whose elements 2 r, 2 r + 1 are features 2 r, 2 r + 1 (r odd, or HIGH: times 16)
+template <bool HIGH>
 __device__ __forceinline__ f16x8 kv4_k_operand(uint32_t x) {
+    constexpr uint32_t lo = 0x000f000fu, hi = 0x00f000f0u;
     const uint32_t y = x >> 8;
-    u32x4 r = {x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u};
+    u32x4 r = {HIGH ? (x << 4) & hi : x & lo, x & hi, HIGH ? (x >> 4) & hi : y & lo, y & hi};
     return __builtin_bit_cast(f16x8, r);
 }
-// two V dwords (4 tokens of tile 2 ks, 4 of tile 2 ks + 1) -> operands of feature n and of feature 16 + n (times 16);
-// the four tokens of a dword come in the order 0 2 1 3
+// two V dwords (4 tokens of tile 2 ks, 4 of tile 2 ks + 1) -> operands of feature n (HIGH: times 16) and of feature 16 + n
+// (times 16); the four tokens of a dword come in the order 0 2 1 3
+template <bool HIGH>
 __device__ __forceinline__ void kv4_v_operands(uint32_t x0, uint32_t x1, f16x8& lo, f16x8& hi) {
+    constexpr uint32_t ml = 0x000f000fu, mh = 0x00f000f0u;
     const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
-    u32x4 l = {x0 & 0x000f000fu, y0 & 0x000f000fu, x1 & 0x000f000fu, y1 & 0x000f000fu};
-    u32x4 h = {x0 & 0x00f000f0u, y0 & 0x00f000f0u, x1 & 0x00f000f0u, y1 & 0x00f000f0u};
+    u32x4 l = {x0 & ml, y0 & ml, x1 & ml, y1 & ml};
+    if (HIGH) l = u32x4{(x0 << 4) & mh, (x0 >> 4) & mh, (x1 << 4) & mh, (x1 >> 4) & mh};
+    u32x4 h = {x0 & mh, y0 & mh, x1 & mh, y1 & mh};
     lo = __builtin_bit_cast(f16x8, l);
     hi = __builtin_bit_cast(f16x8, h);
 }
 __device__ __forceinline__ f32x4 kv4_mfma(f16x8 a, f16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
+
+// Makes a product the fp32 number it is: left alone, the compiler rounds it to fp16 here in one step and there in two, and the
+// second part is now and then the rest of another first part.
+__device__ __forceinline__ void kv4_pin(float& y) { asm volatile("" : "+v"(y)); }
+
+// 2^x of a whole number: references of exponents are whole, so that moving one rounds no sum (codes' and zeros' shares of
+// the context cancel: rounded apart, an fp32 result of 1000 tokens was off by 1e-5)
+__device__ __forceinline__ float kv4_pow2(float x) { return __builtin_amdgcn_ldexpf(1.f, (int)fmaxf(x, -512.f)); }
 
 // the product of this lane's quad, by two conditions (four nested ones become branches)
 __device__ __forceinline__ float kv4_own(float a, float b, float c, float d, bool odd, bool upper) {
@@ -118,7 +137,7 @@ struct Kv4Work {            // what a block works on: query rows q0 .. of (sente
 // The features of a query row that this lane multiplies (8 of every group), and the row's scaling.
 template <typename T, int NG, int PARTS>
 struct Kv4Query {
-    f16x8 op[PARTS][NG];        // fp16 parts of q * 2^up; where the code is 16 times as large, a 16th
+    f16x8 op[PARTS][NG];        // fp16 parts of q * 2^up; where the code is 16 times as large, a 16th (fp32: everywhere)
     float sum[NG];              // sum of q over the group, every lane of the row
     int up;
     __device__ __forceinline__ void load(const T* src, bool have, int dh, int quad) {
@@ -151,7 +170,7 @@ struct Kv4Query {
         for (int g = 0; g < NG; ++g)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                float y = __builtin_amdgcn_ldexpf(x[g][e], ((e >> 1) & 1) ? up - 4 : up);
+                float y = __builtin_amdgcn_ldexpf(x[g][e], sizeof(T) == 4 || ((e >> 1) & 1) ? up - 4 : up);
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p) {
                     const f16 h = (f16)y;
@@ -176,7 +195,7 @@ __device__ __forceinline__ void kv4_finish(const Kv4AttnArgs& a, const Kv4Work& 
         for (int k = 0; k < W; ++k) {
             const float mk = om[k][r][DP], lk = om[k][r][DP + 1];
             // a wave that saw nothing has nothing to add (its maximum is minus infinity, like the joint one may be)
-            const float f = mk == -INFINITY && lk == 0.f ? 0.f : __builtin_amdgcn_exp2f(mk - top);
+            const float f = mk == -INFINITY && lk == 0.f ? 0.f : kv4_pow2(mk - top);
             sum = fmaf(f, lk, sum);
             o0 = fmaf(f, om[k][r][c], o0);
             o1 = fmaf(f, om[k][r][c + 1], o1);
@@ -258,7 +277,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
         }
     }
 
-    // m: the running maximum (up to 8 behind), ref: what exponents are taken relative to, m - 7 + log2 of the V scales' bound;
+    // m: the running maximum (up to 8 behind), ref: what exponents are taken relative to, ceil(m) - 7 + log2 of the V scales' bound;
     // every sum of a row is in units of 2^ref, so that nothing but ref remembers either
     float m[R], ref[R], l[R], zs[R][NG], vtop = 0.f;
     f32x4 acc[2 * NG];
@@ -276,11 +295,48 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
     const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
     const bool odd = quad & 1, upper = quad & 2;
 
+    // Codes' and zeros' shares of the context nearly cancel where values are spread about zero, more so the more tokens there
+    // are: fp32 calls add them up, and set them aside, every KV4_SETTLE blocks (31 blocks a wave: 1e-5 of the result
+    // without, 5e-6 with it; every 4 blocks 2e-6, a fifth slower).
+    float lsum[R], at_ref[R];
+    bool settled = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) lsum[r] = at_ref[r] = 0.f;
+    auto settle = [&]() {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float f = settled ? kv4_pow2(at_ref[r] - ref[r]) : 0.f;
+            lsum[r] = fmaf(lsum[r], f, wave_sum(l[r]));
+            l[r] = 0.f;
+            at_ref[r] = ref[r];
+            float zt[NG];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                zt[g] = wave_sum(zs[r][g]);
+                zs[r][g] = 0.f;
+            }
+#pragma unroll
+            for (int c = 0; c < 2 * NG; ++c) {
+                float u = acc[c][r];
+                if (PARTS == 2) u += __shfl_xor(u, 16);             // quads 0 and 1
+                u = fmaf(u, F32 || (c & 1) ? 0x1p20f : 0x1p24f, zt[c >> 1]);
+                if (quad == 0) {
+                    if (settled) u = fmaf(om[w][r][c * 16 + n], f, u);
+                    om[w][r][c * 16 + n] = u;
+                }
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 2 * NG; ++c) acc[c] = zero4;
+        settled = true;
+    };
+
     const uint8_t* ahead = base + (int64_t)(wk.first + w) * kv4_block_bytes(NG);
     if (!early && wk.first + w < wk.last) {
         cur.load_k(ahead, lane);
         cur.load_v(ahead, lane);
     }
+    int until = KV4_SETTLE;
     for (int blk = wk.first + w; blk < wk.last; blk += W) {
         const bool more = blk + W < wk.last;
         ahead += W * kv4_block_bytes(NG);
@@ -302,7 +358,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
             f32x4 d[4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const f16x8 kop = kv4_k_operand(cur.k[(t * NG + g) >> 2][(t * NG + g) & 3]);
+                const f16x8 kop = kv4_k_operand<F32>(cur.k[(t * NG + g) >> 2][(t * NG + g) & 3]);
                 d[t] = kv4_mfma(qop[0][g], kop, zero4);
                 if constexpr (PARTS == 2 && !QROWS) d[t] = kv4_mfma(qop[PARTS - 1][g], kop, d[t]);
             }
@@ -335,8 +391,8 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 m[r] = fmaxf(m[r], wave_max(s[r]));
-                const float moved = m[r] + e;
-                f[r] = __builtin_amdgcn_exp2f(ref[r] - moved);
+                const float moved = ceilf(m[r]) + e;
+                f[r] = kv4_pow2(ref[r] - moved);
                 ref[r] = moved;
                 l[r] *= f[r];
 #pragma unroll
@@ -353,6 +409,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
             for (int g = 0; g < NG; ++g) {
                 const uint32_t mvr = mv[g] & mask[r];
                 float y = p * kv4_scale(mvr);
+                if (F32) kv4_pin(y);
                 zs[r][g] = fmaf(p, kv4_zero(mvr), zs[r][g]);
 #pragma unroll
                 for (int part = 0; part < PARTS; ++part) {
@@ -366,37 +423,35 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
         // rows 4 part + r; the rows of absent parts and queries repeat others and are not used
         const int row = R == 1 ? (PARTS == 2 ? (n >> 2) & 1 : 0) : (PARTS == 2 ? n & 7 : n & 3);
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+        for (int g = 0; g < NG; ++g) {
+            f32x4 c0 = F32 ? zero4 : acc[2 * g], c1 = F32 ? zero4 : acc[2 * g + 1];
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
+            for (int ks = 0; ks < 2; ++ks) {
                 const int d = (ks * NG + g) * 2;
                 f16x8 lo, hi;
-                kv4_v_operands(cur.v[d >> 2][d & 3], cur.v[d >> 2][(d & 3) + 1], lo, hi);
+                kv4_v_operands<F32>(cur.v[d >> 2][d & 3], cur.v[d >> 2][(d & 3) + 1], lo, hi);
                 const u32x4 raw = *reinterpret_cast<const u32x4*>(&ps[g][row][ks * 32 + quad * 8]);
                 const f16x8 pop = __builtin_bit_cast(f16x8, raw);
-                acc[2 * g] = kv4_mfma(pop, lo, acc[2 * g]);
-                acc[2 * g + 1] = kv4_mfma(pop, hi, acc[2 * g + 1]);
+                c0 = kv4_mfma(pop, lo, c0);
+                c1 = kv4_mfma(pop, hi, c1);
             }
+            acc[2 * g] = F32 ? acc[2 * g] + c0 : c0;
+            acc[2 * g + 1] = F32 ? acc[2 * g + 1] + c1 : c1;
+        }
         __builtin_amdgcn_wave_barrier();
         if (more) cur.load_v(ahead, lane);
+        if (F32 && --until == 0) {
+            settle();
+            until = KV4_SETTLE;
+        }
     }
 
+    settle();
+    if (lane == 0) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const float lt = wave_sum(l[r]);
-        float zt[NG];
-#pragma unroll
-        for (int g = 0; g < NG; ++g) zt[g] = wave_sum(zs[r][g]);
-#pragma unroll
-        for (int c = 0; c < 2 * NG; ++c) {
-            float u = acc[c][r];
-            if (PARTS == 2) u += __shfl_xor(u, 16);             // quads 0 and 1
-            u = fmaf(u, (c & 1) ? 0x1p20f : 0x1p24f, zt[c >> 1]);
-            if (quad == 0) om[w][r][c * 16 + n] = u;
-        }
-        if (lane == 0) {
+        for (int r = 0; r < R; ++r) {
             om[w][r][DP] = m[r] == KV4_NONE ? -INFINITY : ref[r];
-            om[w][r][DP + 1] = lt;
+            om[w][r][DP + 1] = lsum[r];
         }
     }
     if (W > 1) __syncthreads();
@@ -460,6 +515,11 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
     float vtop = 0.f;                            // the largest V scale met; scales are taken times 2^-vexp, which bounds it
     int vexp = 0;
     f32x4 acc[2 * NG], accz = {0.f, 0.f, 0.f, 0.f};         // accz: quad 0: sum p z_g, quad 1: sum p
+    // fp32: a product of two 11-bit numbers fills the 24 bits that the matrix cores align a sum of 32 to, and what falls off
+    // is cut, not rounded; against codes (4 bits) nothing falls off, against zeros it would show (1.5e-5 of the result)
+    float zs[F32 ? NG : 1];
+#pragma unroll
+    for (int g = 0; g < (F32 ? NG : 1); ++g) zs[g] = 0.f;
 #pragma unroll
     for (int c = 0; c < 2 * NG; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
     const uint8_t* base = a.data + (int64_t)wk.bh * a.blocks * kv4_block_bytes(NG);
@@ -476,7 +536,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
             f32x4 d[NG];
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const f16x8 kop = kv4_k_operand(cur.k[(t * NG + g) >> 2][(t * NG + g) & 3]);
+                const f16x8 kop = kv4_k_operand<F32>(cur.k[(t * NG + g) >> 2][(t * NG + g) & 3]);
                 d[g] = kv4_mfma(kop, q.op[0][g], zero4);
                 if constexpr (PARTS == 2) d[g] = kv4_mfma(kop, q.op[PARTS - 1][g], d[g]);
             }
@@ -516,11 +576,14 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
             // by how much this row's reference moves: up, or wherever its first tokens are
-            const float up = !fresh ? fmaxf(top - KV4_UP, 0.f) : top > -INFINITY ? top - KV4_UP : 0.f;
-            const float f = fresh ? 1.f : __builtin_amdgcn_exp2f(-up);
+            const float to = ceilf(top - KV4_UP);
+            const float up = !fresh ? fmaxf(to, 0.f) : top > -INFINITY ? to : 0.f;
+            const float f = fresh ? 1.f : kv4_pow2(-up);
             fresh = fresh && !(top > -INFINITY);
             m += up;
             accz *= f;
+#pragma unroll
+            for (int g = 0; g < (F32 ? NG : 1); ++g) zs[g] *= f;
 #pragma unroll
             for (int c = 0; c < 2 * NG; ++c) acc[c] *= f * shrink;
 #pragma unroll
@@ -560,20 +623,34 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
                     }
                 }
             u32x4 zop = {one2, one2, one2, one2};
-            if (n < NG) zop = *reinterpret_cast<const u32x4*>(&my.vz[n < NG ? n : 0][32 * ks + 8 * quad]);
+            if (!F32 && n < NG) zop = *reinterpret_cast<const u32x4*>(&my.vz[n < NG ? n : 0][32 * ks + 8 * quad]);
 #pragma unroll
             for (int part = 0; part < PARTS; ++part) accz = kv4_mfma(__builtin_bit_cast(f16x8, zop), pop[part], accz);
+        }
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
+        for (int g = 0; g < NG; ++g) {
+            f32x4 c[PARTS][2];                   // one accumulator a part: the smaller part's sums would be cut in the larger's
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) {
+                c[part][0] = F32 ? zero4 : acc[2 * g];
+                c[part][1] = F32 ? zero4 : acc[2 * g + 1];
+            }
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                f16x8 pop[PARTS];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int t = 2 * ks + h;
                     const f32x4 v4 = *reinterpret_cast<const f32x4*>(&my.vs[g][16 * t + 4 * quad]);
+                    uint32_t z2[2] = {0u, 0u};
+                    if (F32) __builtin_memcpy(z2, __builtin_assume_aligned(&my.vz[g][32 * ks + 8 * quad + 4 * h], 8), 8);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int r = (j >> 1) | ((j & 1) << 1);
+                        if (F32) zs[F32 ? g : 0] = fmaf(s[t][r], kv4_half((z2[j >> 1] >> (16 * (j & 1))) & 0xffffu), zs[F32 ? g : 0]);
                         float y = s[t][r] * v4[r];
                         if (EDGE) y = 16 * t + 4 * quad + r < see ? y : 0.f;            // a scale may be NaN
+                        if (F32) kv4_pin(y);
 #pragma unroll
                         for (int part = 0; part < PARTS; ++part) {
                             const f16 b = (f16)y;
@@ -584,15 +661,46 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
                 }
                 const int d = (ks * NG + g) * 2;
                 f16x8 lo, hi;
-                kv4_v_operands(cur.v[d >> 2][d & 3], cur.v[d >> 2][(d & 3) + 1], lo, hi);
+                kv4_v_operands<F32>(cur.v[d >> 2][d & 3], cur.v[d >> 2][(d & 3) + 1], lo, hi);
 #pragma unroll
                 for (int part = 0; part < PARTS; ++part) {
-                    acc[2 * g] = kv4_mfma(lo, pop[part], acc[2 * g]);
-                    acc[2 * g + 1] = kv4_mfma(hi, pop[part], acc[2 * g + 1]);
+                    c[part][0] = kv4_mfma(lo, pop[part], c[part][0]);
+                    c[part][1] = kv4_mfma(hi, pop[part], c[part][1]);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) acc[2 * g + h] = F32 ? acc[2 * g + h] + (c[0][h] + c[PARTS - 1][h]) : c[0][h];
         }
+    };
+
+    float lsum = 0.f, at_m = 0.f;                // lsum: of use in quad 1
+    bool settled = false;
+    auto settle = [&]() {                        // as in kv4_few_kernel
+        const float f = settled ? kv4_pow2(at_m - m) : 0.f, unit = __builtin_amdgcn_ldexpf(1.f, 24 + vexp);
+        lsum = fmaf(lsum, f, accz[0]);
+        at_m = m;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            float z = F32 ? zs[F32 ? g : 0] : __shfl(accz[g], n);
+            if (F32) {
+                z += __shfl_xor(z, 16);
+                z += __shfl_xor(z, 32);
+                zs[F32 ? g : 0] = 0.f;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float& o = om[w][n][g * 32 + h * 16 + quad * 4 + r];
+                    const float u = fmaf(acc[2 * g + h][r], F32 || h ? unit / 16.f : unit, z);
+                    o = settled ? fmaf(o, f, u) : u;
+                }
+        }
+#pragma unroll
+        for (int c = 0; c < 2 * NG; ++c) acc[c] = zero4;
+        accz = zero4;
+        settled = true;
     };
 
     const uint8_t* ahead = base + (int64_t)(wk.first + w) * kv4_block_bytes(NG);
@@ -600,6 +708,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
         cur.load_k(ahead, lane);
         cur.load_v(ahead, lane);
     }
+    int until = KV4_SETTLE;
     for (int blk = wk.first + w; blk < wk.last; blk += W) {
         const bool more = blk + W < wk.last;
         ahead += W * kv4_block_bytes(NG);
@@ -624,21 +733,16 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
         }
         __builtin_amdgcn_wave_barrier();
         if (more) cur.load_v(ahead, lane);
+        if (F32 && --until == 0) {
+            settle();
+            until = KV4_SETTLE;
+        }
     }
 
-    const float unit = __builtin_amdgcn_ldexpf(1.f, 24 + vexp);
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-        const float z = __shfl(accz[g], n);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                om[w][n][g * 32 + h * 16 + quad * 4 + r] = fmaf(acc[2 * g + h][r], h ? unit / 16.f : unit, z);
-    }
+    settle();
     if (quad == 1) {
         om[w][n][DP] = fresh ? -INFINITY : m;
-        om[w][n][DP + 1] = accz[0];
+        om[w][n][DP + 1] = lsum;
     }
     if (W > 1) __syncthreads();
     else __builtin_amdgcn_wave_barrier();
@@ -659,7 +763,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a) {
     float sum = 0.f;
     for (int s = threadIdx.x; s < a.splits; s += 256) {
         const float2 x = ml[s];
-        const float f = x.x == -INFINITY && x.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x.x - top);
+        const float f = x.x == -INFINITY && x.y == 0.f ? 0.f : kv4_pow2(x.x - top);
         fac[s] = f;
         sum = fmaf(f, x.y, sum);
     }
