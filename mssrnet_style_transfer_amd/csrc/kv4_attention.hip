@@ -16,8 +16,10 @@
 // V scale met so far (rounded up to a power of two; when it grows, the sums shrink), with p up to 2^8 (below) and 7 bits
 // on top, so that what is 2^-21 of the largest still has all its bits and the rest is off by at most 2^-32 of it.
 //
-// A product's sums are cut, not rounded, where they meet an accumulator that has outgrown them by more than 24 bits less
-// their own; fp32 calls therefore start every block of 64 tokens from zero and add it up by rounding additions.
+// Where values are spread about zero, codes' and zeros' shares of the context nearly cancel, the more so the more tokens
+// there are, and a product's sums are cut, not rounded, where they meet an accumulator that has outgrown them.  fp32 calls
+// therefore take 7.5 from every code (one more product against a constant) and add 7.5 s to every zero, and start each
+// block of 64 tokens from zero, added up by rounding additions: 1000 .. 16000 tokens of mean zero come out within 1e-6.
 //
 // A wave takes 64 tokens at a time; the running maximum moves only when a score passes it by more than 8 (then every
 // sum is rescaled), so that a block of tokens costs one comparison and no cross-lane reduction.  The W waves of a block
@@ -46,7 +48,7 @@ struct Kv4AttnArgs {
 constexpr float KV4_LAZY = 8.f;          // log2 of how far a probability may pass 1 before a rescale
 constexpr float KV4_UP = 7.f;            // log2 of what probabilities are held times
 constexpr float KV4_NONE = -3e38f;       // the reference of a row that has seen no token: 2^(-inf - KV4_NONE) is 0
-constexpr int KV4_SETTLE = 16;           // blocks between two settlings of fp32 sums (kv4_few_kernel)
+constexpr float KV4_MID = 7.5f;          // what fp32 calls take from codes and add, times the scale, to zeros
 constexpr int KV4_MAX_SPLITS = 512;
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -70,6 +72,12 @@ __device__ __forceinline__ void kv4_v_operands(uint32_t x0, uint32_t x1, f16x8& 
     u32x4 h = {x0 & mh, y0 & mh, x1 & mh, y1 & mh};
     lo = __builtin_bit_cast(f16x8, l);
     hi = __builtin_bit_cast(f16x8, h);
+}
+// -KV4_MID times 16 in every place
+__device__ __forceinline__ f16x8 kv4_mid() {
+    constexpr uint32_t w = 0x80788078u;          // -120 * 2^-24, twice
+    u32x4 r = {w, w, w, w};
+    return __builtin_bit_cast(f16x8, r);
 }
 __device__ __forceinline__ f32x4 kv4_mfma(f16x8 a, f16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -295,48 +303,11 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
     const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
     const bool odd = quad & 1, upper = quad & 2;
 
-    // Codes' and zeros' shares of the context nearly cancel where values are spread about zero, more so the more tokens there
-    // are: fp32 calls add them up, and set them aside, every KV4_SETTLE blocks (31 blocks a wave: 1e-5 of the result
-    // without, 5e-6 with it; every 4 blocks 2e-6, a fifth slower).
-    float lsum[R], at_ref[R];
-    bool settled = false;
-#pragma unroll
-    for (int r = 0; r < R; ++r) lsum[r] = at_ref[r] = 0.f;
-    auto settle = [&]() {
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const float f = settled ? kv4_pow2(at_ref[r] - ref[r]) : 0.f;
-            lsum[r] = fmaf(lsum[r], f, wave_sum(l[r]));
-            l[r] = 0.f;
-            at_ref[r] = ref[r];
-            float zt[NG];
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                zt[g] = wave_sum(zs[r][g]);
-                zs[r][g] = 0.f;
-            }
-#pragma unroll
-            for (int c = 0; c < 2 * NG; ++c) {
-                float u = acc[c][r];
-                if (PARTS == 2) u += __shfl_xor(u, 16);             // quads 0 and 1
-                u = fmaf(u, F32 || (c & 1) ? 0x1p20f : 0x1p24f, zt[c >> 1]);
-                if (quad == 0) {
-                    if (settled) u = fmaf(om[w][r][c * 16 + n], f, u);
-                    om[w][r][c * 16 + n] = u;
-                }
-            }
-        }
-#pragma unroll
-        for (int c = 0; c < 2 * NG; ++c) acc[c] = zero4;
-        settled = true;
-    };
-
     const uint8_t* ahead = base + (int64_t)(wk.first + w) * kv4_block_bytes(NG);
     if (!early && wk.first + w < wk.last) {
         cur.load_k(ahead, lane);
         cur.load_v(ahead, lane);
     }
-    int until = KV4_SETTLE;
     for (int blk = wk.first + w; blk < wk.last; blk += W) {
         const bool more = blk + W < wk.last;
         ahead += W * kv4_block_bytes(NG);
@@ -410,7 +381,8 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
                 const uint32_t mvr = mv[g] & mask[r];
                 float y = p * kv4_scale(mvr);
                 if (F32) kv4_pin(y);
-                zs[r][g] = fmaf(p, kv4_zero(mvr), zs[r][g]);
+                const float z = F32 ? fmaf(KV4_MID, kv4_scale(mvr), kv4_zero(mvr)) : kv4_zero(mvr);
+                zs[r][g] = fmaf(p, z, zs[r][g]);
 #pragma unroll
                 for (int part = 0; part < PARTS; ++part) {
                     const f16 h = (f16)y;
@@ -424,7 +396,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
         const int row = R == 1 ? (PARTS == 2 ? (n >> 2) & 1 : 0) : (PARTS == 2 ? n & 7 : n & 3);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            f32x4 c0 = F32 ? zero4 : acc[2 * g], c1 = F32 ? zero4 : acc[2 * g + 1];
+            f32x4 c0 = F32 ? zero4 : acc[2 * g], c1 = F32 ? zero4 : acc[2 * g + 1], mid = zero4;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
                 const int d = (ks * NG + g) * 2;
@@ -434,24 +406,31 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
                 const f16x8 pop = __builtin_bit_cast(f16x8, raw);
                 c0 = kv4_mfma(pop, lo, c0);
                 c1 = kv4_mfma(pop, hi, c1);
+                if (F32) mid = kv4_mfma(pop, kv4_mid(), mid);
             }
-            acc[2 * g] = F32 ? acc[2 * g] + c0 : c0;
-            acc[2 * g + 1] = F32 ? acc[2 * g + 1] + c1 : c1;
+            acc[2 * g] = F32 ? acc[2 * g] + (c0 + mid) : c0;
+            acc[2 * g + 1] = F32 ? acc[2 * g + 1] + (c1 + mid) : c1;
         }
         __builtin_amdgcn_wave_barrier();
         if (more) cur.load_v(ahead, lane);
-        if (F32 && --until == 0) {
-            settle();
-            until = KV4_SETTLE;
-        }
     }
 
-    settle();
-    if (lane == 0) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
+    for (int r = 0; r < R; ++r) {
+        const float lt = wave_sum(l[r]);
+        float zt[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) zt[g] = wave_sum(zs[r][g]);
+#pragma unroll
+        for (int c = 0; c < 2 * NG; ++c) {
+            float u = acc[c][r];
+            if (PARTS == 2) u += __shfl_xor(u, 16);             // quads 0 and 1
+            u = fmaf(u, F32 || (c & 1) ? 0x1p20f : 0x1p24f, zt[c >> 1]);
+            if (quad == 0) om[w][r][c * 16 + n] = u;
+        }
+        if (lane == 0) {
             om[w][r][DP] = m[r] == KV4_NONE ? -INFINITY : ref[r];
-            om[w][r][DP + 1] = lsum[r];
+            om[w][r][DP + 1] = lt;
         }
     }
     if (W > 1) __syncthreads();
@@ -478,6 +457,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
         uint16_t ks[NG][KV4_TOK];           // K scales
         uint16_t vz[NG][KV4_TOK];           // V zeros in the operand's token order
         uint2 kz[KV4_TOK];                  // K zeros, groups 0..3
+        float vm[F32 ? NG : 1][KV4_TOK];    // fp32 calls: V zeros and KV4_MID V scales
     };
     __shared__ __align__(16) Token tk[kv4_waves(W)];
     __shared__ float om_[kv4_waves(W) / W][W][16][DP + 4];
@@ -515,8 +495,6 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
     float vtop = 0.f;                            // the largest V scale met; scales are taken times 2^-vexp, which bounds it
     int vexp = 0;
     f32x4 acc[2 * NG], accz = {0.f, 0.f, 0.f, 0.f};         // accz: quad 0: sum p z_g, quad 1: sum p
-    // fp32: a product of two 11-bit numbers fills the 24 bits that the matrix cores align a sum of 32 to, and what falls off
-    // is cut, not rounded; against codes (4 bits) nothing falls off, against zeros it would show (1.5e-5 of the result)
     float zs[F32 ? NG : 1];
 #pragma unroll
     for (int g = 0; g < (F32 ? NG : 1); ++g) zs[g] = 0.f;
@@ -597,6 +575,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
             const float vz = kv4_zero(mv[g]);
             my.vs[g][lane] = kv4_scale(mv[g]) * vmul;
             my.vz[g][col] = vz == vz ? (uint16_t)(mv[g] >> 16) : (uint16_t)0;
+            if (F32) my.vm[F32 ? g : 0][lane] = vz == vz ? fmaf(KV4_MID, kv4_scale(mv[g]), vz) : 0.f;
         }
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -629,7 +608,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
         }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            f32x4 c[PARTS][2];                   // one accumulator a part: the smaller part's sums would be cut in the larger's
+            f32x4 c[PARTS][2], mid = zero4;      // one accumulator a part: the smaller part's sums would be cut in the larger's
 #pragma unroll
             for (int part = 0; part < PARTS; ++part) {
                 c[part][0] = F32 ? zero4 : acc[2 * g];
@@ -642,12 +621,12 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
                 for (int h = 0; h < 2; ++h) {
                     const int t = 2 * ks + h;
                     const f32x4 v4 = *reinterpret_cast<const f32x4*>(&my.vs[g][16 * t + 4 * quad]);
-                    uint32_t z2[2] = {0u, 0u};
-                    if (F32) __builtin_memcpy(z2, __builtin_assume_aligned(&my.vz[g][32 * ks + 8 * quad + 4 * h], 8), 8);
+                    f32x4 z4 = zero4;
+                    if (F32) z4 = *reinterpret_cast<const f32x4*>(&my.vm[F32 ? g : 0][16 * t + 4 * quad]);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int r = (j >> 1) | ((j & 1) << 1);
-                        if (F32) zs[F32 ? g : 0] = fmaf(s[t][r], kv4_half((z2[j >> 1] >> (16 * (j & 1))) & 0xffffu), zs[F32 ? g : 0]);
+                        if (F32) zs[F32 ? g : 0] = fmaf(s[t][r], z4[r], zs[F32 ? g : 0]);
                         float y = s[t][r] * v4[r];
                         if (EDGE) y = 16 * t + 4 * quad + r < see ? y : 0.f;            // a scale may be NaN
                         if (F32) kv4_pin(y);
@@ -666,41 +645,13 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
                 for (int part = 0; part < PARTS; ++part) {
                     c[part][0] = kv4_mfma(lo, pop[part], c[part][0]);
                     c[part][1] = kv4_mfma(hi, pop[part], c[part][1]);
+                    if (F32) mid = kv4_mfma(kv4_mid(), pop[part], mid);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) acc[2 * g + h] = F32 ? acc[2 * g + h] + (c[0][h] + c[PARTS - 1][h]) : c[0][h];
+            for (int h = 0; h < 2; ++h) acc[2 * g + h] = F32 ? acc[2 * g + h] + (c[0][h] + mid + c[PARTS - 1][h]) : c[0][h];
         }
-    };
-
-    float lsum = 0.f, at_m = 0.f;                // lsum: of use in quad 1
-    bool settled = false;
-    auto settle = [&]() {                        // as in kv4_few_kernel
-        const float f = settled ? kv4_pow2(at_m - m) : 0.f, unit = __builtin_amdgcn_ldexpf(1.f, 24 + vexp);
-        lsum = fmaf(lsum, f, accz[0]);
-        at_m = m;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            float z = F32 ? zs[F32 ? g : 0] : __shfl(accz[g], n);
-            if (F32) {
-                z += __shfl_xor(z, 16);
-                z += __shfl_xor(z, 32);
-                zs[F32 ? g : 0] = 0.f;
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float& o = om[w][n][g * 32 + h * 16 + quad * 4 + r];
-                    const float u = fmaf(acc[2 * g + h][r], F32 || h ? unit / 16.f : unit, z);
-                    o = settled ? fmaf(o, f, u) : u;
-                }
-        }
-#pragma unroll
-        for (int c = 0; c < 2 * NG; ++c) acc[c] = zero4;
-        accz = zero4;
-        settled = true;
     };
 
     const uint8_t* ahead = base + (int64_t)(wk.first + w) * kv4_block_bytes(NG);
@@ -708,7 +659,6 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
         cur.load_k(ahead, lane);
         cur.load_v(ahead, lane);
     }
-    int until = KV4_SETTLE;
     for (int blk = wk.first + w; blk < wk.last; blk += W) {
         const bool more = blk + W < wk.last;
         ahead += W * kv4_block_bytes(NG);
@@ -733,16 +683,25 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
         }
         __builtin_amdgcn_wave_barrier();
         if (more) cur.load_v(ahead, lane);
-        if (F32 && --until == 0) {
-            settle();
-            until = KV4_SETTLE;
-        }
     }
 
-    settle();
+    const float unit = __builtin_amdgcn_ldexpf(1.f, 24 + vexp);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        float z = F32 ? zs[F32 ? g : 0] : __shfl(accz[g], n);
+        if (F32) {
+            z += __shfl_xor(z, 16);
+            z += __shfl_xor(z, 32);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                om[w][n][g * 32 + h * 16 + quad * 4 + r] = fmaf(acc[2 * g + h][r], F32 || h ? unit / 16.f : unit, z);
+    }
     if (quad == 1) {
         om[w][n][DP] = fresh ? -INFINITY : m;
-        om[w][n][DP + 1] = lsum;
+        om[w][n][DP + 1] = accz[0];
     }
     if (W > 1) __syncthreads();
     else __builtin_amdgcn_wave_barrier();
