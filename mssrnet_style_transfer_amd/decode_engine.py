@@ -24,6 +24,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from . import ops
+from .token_control import pick_token
 from .weight_pack import JobTable
 
 N_HEAD_PARAMS = 5
@@ -759,7 +760,7 @@ def soft_decode(model, cfg, memory_bank, src_lengths, steps, eval_rows=0, forced
     return _SoftDecode.apply(spec, mem, *params)
 
 
-def greedy_decode_ids(model, cfg, memory_bank, src_lengths, max_length, check_every=4, compact_below=0.75):
+def greedy_decode_ids(model, cfg, memory_bank, src_lengths, max_length, check_every=4, compact_below=0.75, control=None):
     """Greedy search with beam 1 on the decode engine: token ids [steps, B] (int32; steps <= max_length,
     the loop stops once every sentence has produced </s>) -- the step loop of
     onmt/translate/translator_wh.py:709-746 with GreedySearch.advance (greedy_search.py:135-165).
@@ -769,7 +770,11 @@ def greedy_decode_ids(model, cfg, memory_bank, src_lengths, max_length, check_ev
     ``check_every`` steps, where the loop reads the done flags anyway) and only once fewer than ``compact_below``
     of the current rows are still running: the survivors' memory bank, self-attention cache rows and last tokens are
     gathered into a smaller plan and the sweep continues on it.  What a row holds after its sentence's first </s> is
-    unspecified (tokens of the steps it kept running, then </s>); the caller cuts each sentence at its first </s>."""
+    unspecified (tokens of the steps it kept running, then </s>); the caller cuts each sentence at its first </s>.
+
+    ``control`` (token_control.TokenControl, no reference counterpart): rules for the logits of every step over the words
+    picked so far -- repetition penalties, biases, per-sentence grammar masks, no repeated n-grams.  A sentence whose
+    rules leave nothing ends (</s>)."""
     lib = L.load()
     params = decoder_params(model)
     dev = memory_bank.device
@@ -785,6 +790,8 @@ def greedy_decode_ids(model, cfg, memory_bank, src_lengths, max_length, check_ev
             plan, bufs = _make_plan(sp, mem.transpose(0, 1).contiguous(), greedy=True)
             ids = torch.zeros(sp.T, sp.B, dtype=torch.int32, device=dev)
             plan.ids, plan.greedy = ids.data_ptr(), 1
+            if control is not None:
+                plan.n_chunks = 1       # the pick below follows the step on its stream
             return plan, bufs, ids
 
         plan, bufs, ids = new_plan(spec, mem_cur)
@@ -792,6 +799,9 @@ def greedy_decode_ids(model, cfg, memory_bank, src_lengths, max_length, check_ev
         steps = flushed = 0
         for step in range(T):
             L.check(lib.mssr_decode_step_fwd(ctypes.byref(plan), step, L.stream()), "decode_step_fwd")
+            if control is not None:     # the step's own argmax gives way to the controlled one; the next step reads ids[step]
+                pick_token(bufs["logits"][:, :spec.pack.V], control, ids[:step].t() if step else None, empty=cfg.eos_idx,
+                           out=ids[step])
             steps = step + 1
             if steps % check_every and steps != T:
                 continue
@@ -812,6 +822,8 @@ def greedy_decode_ids(model, cfg, memory_bank, src_lengths, max_length, check_ev
                 # the survivors' self-attention keys / values of the steps so far, and their last tokens
                 bufs2["qkv"].view(NL, n_live, T, d3)[:, :, :steps] = bufs["qkv"].view(NL, Bc, T, d3)[:, :, :steps].index_select(1, keep)
                 ids2[:steps] = ids[:steps].index_select(1, keep)
+                if control is not None:
+                    control = control.rows(keep, rows.numel())
                 rows = rows.index_select(0, keep)
                 plan, bufs, ids, spec = plan2, bufs2, ids2, sp
     return out[:steps]

@@ -19,6 +19,7 @@ import torch
 import torch.nn as nn
 
 from .. import ops
+from ..kv_cache import KVCache4
 from ..modules.multi_headed_attn import MultiHeadedAttention
 from ..modules.position_ffn import PositionwiseFeedForward
 from ..utils.misc import padding_mask
@@ -85,7 +86,7 @@ class TransformerDecoderLayer(nn.Module):
             raise NotImplementedError("guided alignment (with_align) is not part of the MSSRNet path")
         out, probs = self._forward(inputs, memory_bank, src_pad_mask, tgt_pad_mask, layer_cache=layer_cache,
                                    step=step)
-        return out, probs[:, 0].contiguous(), None
+        return out, None if probs is None else probs[:, 0].contiguous(), None
 
     def update_dropout(self, dropout, attention_dropout):
         for attn in (self.self_attn, self.context_attn):
@@ -123,13 +124,31 @@ class TransformerDecoder(DecoderBase):
                    alignment_heads=opt.alignment_heads)
 
     # ---- decoding state: {"src": [Ls,B,1] ids, "cache": {"layer_i": {four tensors [B,H,len,dh]}} | None}
-    def init_state(self, src, memory_bank, enc_hidden):
+    def init_state(self, src, memory_bank, enc_hidden, kv_bits=None, max_steps=None):
+        """``kv_bits=4`` (no reference counterpart): the step-by-step decode keeps every layer's keys and values, its own
+        and the memory bank's, in 4 bits (kv_cache.KVCache4: 5 bits a feature with its scales, read as codes); own ones for
+        up to ``max_steps`` tokens.  For decoding under torch.no_grad() in eval mode; attention probabilities are not
+        returned then (``forward`` gives {"std": None})."""
+        if kv_bits not in (None, 4):
+            raise ValueError("kv_bits: None (keys and values as they are) or 4 (got %r)" % (kv_bits,))
+        if kv_bits is not None and (max_steps is None or max_steps < 1):
+            raise ValueError("a 4-bit cache needs max_steps, the tokens a sentence may grow to")
         self.state["src"] = src
         self.state["cache"] = None
+        self.state["kv4_steps"] = None if kv_bits is None else int(max_steps)
 
-    def _init_cache(self, memory_bank):
-        self.state["cache"] = {"layer_%d" % i: dict.fromkeys(_CACHE_SLOTS)
-                               for i in range(len(self.transformer_layers))}
+    def _init_cache(self, memory_bank, memory_lengths=None):
+        steps = self.state.get("kv4_steps")
+        if steps is None:
+            self.state["cache"] = {"layer_%d" % i: dict.fromkeys(_CACHE_SLOTS)
+                                   for i in range(len(self.transformer_layers))}
+            return
+        lengths = memory_lengths.to(memory_bank.device)
+        self.state["cache"] = {
+            "layer_%d" % i: {"self_kv4": KVCache4(memory_bank.size(1), layer.self_attn.head_count,
+                                                  layer.self_attn.dim_per_head, steps, memory_bank.device),
+                             "self_len": 0, "memory_kv4": None, "memory_lengths": lengths}
+            for i, layer in enumerate(self.transformer_layers)}
 
     def map_state(self, fn):
         """Applies ``fn(tensor, batch_dim)`` to the source ids (batch on dim 1) and to every cached
@@ -138,7 +157,9 @@ class TransformerDecoder(DecoderBase):
         self.state["src"] = fn(self.state["src"], 1)
         for layer_cache in (self.state["cache"] or {}).values():
             for slot, held in layer_cache.items():
-                if held is not None:
+                if isinstance(held, KVCache4):
+                    held.map(fn)
+                elif torch.is_tensor(held):
                     layer_cache[slot] = fn(held, 0)
 
     def detach_state(self):
@@ -149,7 +170,7 @@ class TransformerDecoder(DecoderBase):
         if with_align:
             raise NotImplementedError("guided alignment (with_align) is not part of the MSSRNet path")
         if step == 0:
-            self._init_cache(memory_bank)
+            self._init_cache(memory_bank, memory_lengths)
         x = self.embeddings(tgt, step=step).transpose(0, 1).contiguous()          # [B,T,d]
         memory = memory_bank.transpose(0, 1).contiguous()                          # [B,Ls,d]
         # the source width comes from the ids given to init_state, as in the reference (:304)
@@ -170,7 +191,7 @@ class TransformerDecoder(DecoderBase):
             x, top, _ = layer(x, memory, src_pad, tgt_pad, step=step,
                               layer_cache=None if caches is None else caches["layer_%d" % i])
         dec_outs = _norm(self.layer_norm, x).transpose(0, 1).contiguous()
-        return dec_outs, {"std": top.transpose(0, 1).contiguous()}
+        return dec_outs, {"std": None if top is None else top.transpose(0, 1).contiguous()}
 
     def update_dropout(self, dropout, attention_dropout):
         self.embeddings.update_dropout(dropout)

@@ -71,6 +71,9 @@ class KVCache4:
     def nbytes(self):
         return self.data.numel()
 
+    def __getstate__(self):
+        return dict(self.__dict__, _held=None)      # checkpoints and copies hold the data, not its address
+
     def _desc(self):
         """byref of the C descriptor of the present data."""
         if self._held is None or self._held[0] is not self.data:

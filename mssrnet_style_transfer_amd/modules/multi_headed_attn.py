@@ -7,7 +7,7 @@ attribute names (state-dict keys ``linear_{keys,values,query}.{weight,bias}``,
 import torch
 import torch.nn as nn
 
-from .. import ops
+from .. import kv_cache, ops
 
 
 class MultiHeadedAttention(nn.Module):
@@ -34,6 +34,8 @@ class MultiHeadedAttention(nn.Module):
         """key/value/query: [B, len, d] batch-first.  mask: Bool [B,1,Lk] or [B,Lq,Lk], True =
         masked (filled with -1e18 before the fp32 softmax).  Returns (output [B,Lq,d],
         attention [B,H,Lq,Lk] = probabilities BEFORE dropout)."""
+        if layer_cache is not None and "self_kv4" in layer_cache:
+            return self._forward_kv4(key, value, query, layer_cache, attn_type), None
         B = key.size(0)
         H, dh = self.head_count, self.dim_per_head
 
@@ -72,6 +74,34 @@ class MultiHeadedAttention(nn.Module):
         context = ctx.permute(0, 2, 1, 3).reshape(B, Lq, H * dh)     # a view: ctx is stored [B,Lq,H,dh]
         output = self._proj(self.final_linear, context)
         return output, attn
+
+    def _forward_kv4(self, key, value, query, layer_cache, attn_type):
+        """The cached branches over a 4-bit cache (TransformerDecoder.init_state(kv_bits=4)): the new tokens' keys and
+        values, or once the memory bank's, are quantised into it and attended over as codes.  Decoding only: no graph, no
+        dropout, no probabilities.  The memory bank's padding is ``layer_cache["memory_lengths"]``, not a mask."""
+        if self.training and self.dropout.p > 0:
+            raise RuntimeError("a 4-bit cache serves decoding: put the decoder in eval mode")
+        H, dh = self.head_count, self.dim_per_head
+
+        def shape(x):       # [B, len, d] -> [B, H, len, dh] view, no copy
+            return x.view(x.size(0), -1, H, dh).transpose(1, 2)
+
+        q = shape(self._proj(self.linear_query, query))
+        if attn_type == "self":
+            cache, held = layer_cache["self_kv4"], layer_cache["self_len"]
+            cache.write(shape(self._proj(self.linear_keys, query)), shape(self._proj(self.linear_values, query)), held)
+            layer_cache["self_len"] = held = held + q.size(2)
+            ctx = kv_cache.attention(q, cache, held, causal=True)
+        elif attn_type == "context":
+            cache = layer_cache["memory_kv4"]
+            if cache is None:
+                k, v = shape(self._proj(self.linear_keys, key)), shape(self._proj(self.linear_values, value))
+                cache = layer_cache["memory_kv4"] = kv_cache.KVCache4(k.size(0), H, dh, k.size(2), k.device)
+                cache.write(k, v)
+            ctx = kv_cache.attention(q, cache, layer_cache["memory_lengths"])
+        else:
+            raise ValueError("layer_cache needs attn_type 'self' or 'context'")
+        return self._proj(self.final_linear, ctx.permute(0, 2, 1, 3).reshape(q.size(0), -1, H * dh))
 
     def update_dropout(self, dropout):
         self.dropout.p = dropout

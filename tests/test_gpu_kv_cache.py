@@ -379,6 +379,19 @@ def test_map_reorders_sentences(kv):
     assert kv.attention(q[:0], c, 30).shape == (0, 2, 1, 64)
 
 
+def test_copies_and_checkpoints(kv):
+    import copy
+    import pickle
+    c = kv.KVCache4(2, 1, 32, 20)
+    k, q = heads(2, 1, 20, 32, torch.float32, 91), heads(2, 1, 1, 32, torch.float32, 92)
+    c.write(k, k)
+    want = kv.attention(q, c, 20)
+    twin, back = copy.deepcopy(c), pickle.loads(pickle.dumps(c))
+    c.write(k * 2, k * 2)
+    for other in (twin, back):
+        assert other.data.data_ptr() != c.data.data_ptr() and torch.equal(kv.attention(q, other, 20), want)
+
+
 def test_refusals(kv):
     c = kv.KVCache4(2, 2, 64, 40)
     x = torch.zeros(2, 2, 3, 64, device="cuda")
