@@ -3,7 +3,7 @@
 //
 // Per row, in fp32 with every step rounded:
 //   v in the history:  x = x > 0 ? x / repetition : x * repetition
-//   x = x - (frequency * count + presence * (count > 0)),  count over the history from prompt_lengths on
+//   its count, over the history from prompt_lengths on, above 0:  x = x - (frequency * count + presence)
 //   x = x + bias[v];   x = -inf where the mask's bit is 0 or v would complete an n-gram of the history
 // Bound by memory: the logits once, written once or not at all.  A block owns a chunk of a row: it walks the history
 // first and marks the chunk's words in LDS (count, seen, banned; 16 bits a word while counts fit, so that a chunk can be
@@ -18,6 +18,7 @@ constexpr int TC_UNIT = TC_THREADS * 8;          // a chunk is a multiple of thi
 constexpr int TC_LDS = 65536;                    // bytes of marks
 constexpr int64_t TC_MAX_GRID = (1 << 22) - 1;   // blocks of 1024 threads: a grid has fewer than 2^32 threads
 constexpr int64_t TC_MAX_T = 0x3fffffff;
+constexpr int64_t TC_MAX_LD = (int64_t)1 << 36;  // of rows: 2^22 of them stay within 64-bit offsets
 
 // a word's mark: the two top bits of M (16 or 32 bits) are flags, the rest counts
 template <typename M> struct Mark {
@@ -191,7 +192,7 @@ __global__ __launch_bounds__(TC_THREADS, sizeof(M) == 2 ? 8 : 4) void token_cont
                     if (!mk) continue;
                     const uint32_t c = mk & Mark<M>::count;
                     const float z = y[e] > 0.f ? y[e] / rep : y[e] * rep;
-                    y[e] = z - (freq * (float)c + (c ? pres : 0.f));
+                    y[e] = c ? z - (freq * (float)c + pres) : z;     // (an infinite rate leaves the words that it does not count)
                     if (mk & Mark<M>::banned) ban |= 1u << e;
                 }
             }
@@ -270,6 +271,18 @@ static TcShape tc_shape(int64_t B, int64_t V, int64_t T, bool pick) {
     return s;
 }
 
+// New logits take the old ones' place exactly, or share no element with them: apart as wholes, or other columns of equally
+// strided rows.
+static bool tc_apart(const mssr_token_control_desc* d) {
+    const int64_t es = d->dtype == MSSR_F32 ? 4 : 2, x = (int64_t)(intptr_t)d->logits, y = (int64_t)(intptr_t)d->out;
+    if (x == y) return d->B == 1 || d->ld == d->ldo;
+    const int64_t row = d->V * es;
+    if (x + (d->B - 1) * d->ld * es + row <= y || y + (d->B - 1) * d->ldo * es + row <= x) return true;
+    if (d->ld != d->ldo) return false;
+    const int64_t gap = ((y - x) % (d->ld * es) + d->ld * es) % (d->ld * es);
+    return gap >= row && gap <= d->ld * es - row;
+}
+
 template <typename T>
 static void tc_launch(const TokenControlArgs& a, bool wide, unsigned grid, unsigned lds, hipStream_t st) {
     if (wide) token_control_kernel<T, uint32_t><<<grid, TC_THREADS, lds, st>>>(a);
@@ -288,12 +301,14 @@ extern "C" int64_t mssr_token_control_scratch(int64_t B, int64_t V, int64_t T) {
 
 extern "C" int mssr_token_control(const mssr_token_control_desc* d, void* stream) {
     MSSR_REQUIRE(d, "token_control: no descriptor");
-    MSSR_REQUIRE(d->B >= 0 && d->V >= 1 && d->V <= INT32_MAX && d->ld >= d->V, "token_control: logits [%lld, %lld], row stride %lld",
+    MSSR_REQUIRE(d->B >= 0 && d->V >= 1 && d->V <= INT32_MAX && d->ld >= d->V && d->ld <= TC_MAX_LD, "token_control: logits [%lld, %lld], row stride %lld",
                  (long long)d->B, (long long)d->V, (long long)d->ld);
     MSSR_REQUIRE(valid_dtype(d->dtype), "token_control: dtype %d", d->dtype);
     if (d->B == 0) return MSSR_OK;
     MSSR_REQUIRE(d->logits && (d->out || d->ids), "token_control: null operand");
-    MSSR_REQUIRE(!d->out || d->ldo >= d->V, "token_control: row stride %lld of the new logits", (long long)d->ldo);
+    MSSR_REQUIRE(!d->out || (d->ldo >= d->V && d->ldo <= TC_MAX_LD), "token_control: row stride %lld of the new logits", (long long)d->ldo);
+    MSSR_REQUIRE(!d->ids || (d->index_bits & 16) || (d->empty >= INT32_MIN && d->empty <= INT32_MAX),
+                 "token_control: %lld for an empty row does not fit 32-bit picks", (long long)d->empty);
     MSSR_REQUIRE(d->T >= 0 && d->T <= TC_MAX_T, "token_control: history of %lld tokens", (long long)d->T);
     MSSR_REQUIRE(d->ngram >= 0 && d->ngram <= 64, "token_control: n-grams of %d (0 = none, up to 64)", d->ngram);
     MSSR_REQUIRE(!d->allowed || (d->states >= 1 && d->state_mode >= 0 && d->state_mode <= 2 &&
@@ -302,6 +317,7 @@ extern "C" int mssr_token_control(const mssr_token_control_desc* d, void* stream
     const bool hist = d->history && d->T > 0;
     const TcShape s = tc_shape(d->B, d->V, d->T, d->ids != nullptr);
     MSSR_REQUIRE(d->B <= TC_MAX_GRID / s.chunks, "token_control: %lld rows in one call", (long long)d->B);
+    MSSR_REQUIRE(!d->out || tc_apart(d), "token_control: the new logits overlap the old ones without taking their place");
     MSSR_REQUIRE(!d->ids || s.chunks == 1 ||
                      (d->scratch && d->scratch_bytes >= d->B * s.chunks * (int64_t)sizeof(unsigned long long)),
                  "token_control: scratch of %lld bytes is too small", (long long)d->scratch_bytes);

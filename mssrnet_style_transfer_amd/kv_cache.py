@@ -75,10 +75,11 @@ class KVCache4:
         return dict(self.__dict__, _held=None)      # checkpoints and copies hold the data, not its address
 
     def _desc(self):
-        """byref of the C descriptor of the present data."""
-        if self._held is None or self._held[0] is not self.data:
-            d = L.Kv4Cache(self.data.data_ptr(), self.batch, self.capacity, self.heads, self.dim)
-            self._held = (self.data, d, ctypes.byref(d))
+        """byref of the C descriptor of the present data (built again where that has moved or changed its batch)."""
+        at = (self.data.data_ptr(), self.data.shape[0])
+        if self._held is None or self._held[0] != at:
+            d = L.Kv4Cache(*at, self.capacity, self.heads, self.dim)
+            self._held = (at, d, ctypes.byref(d))
         return self._held[2]
 
     def _span(self, who, start, T, counts):

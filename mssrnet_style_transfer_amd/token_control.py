@@ -18,7 +18,7 @@ class TokenControl:
     """The rules of a batch.  In fp32, each step rounded, for every word v of the vocabulary:
 
     1. a word of the history: ``x = x / repetition`` where x > 0, ``x * repetition`` elsewhere;
-    2. ``x - (frequency * count + presence * (count > 0))``, count = how often the history holds it from prompt_lengths on;
+    2. where the history holds it ``count > 0`` times from prompt_lengths on: ``x - (frequency * count + presence)``;
     3. ``x + bias[v]``;
     4. minus infinity where ``allowed`` has no bit for it, or where it would complete an ``ngram``-gram of the history
        (1: no word twice).
@@ -128,7 +128,7 @@ def _call(who, logits, control, history, lengths, prompt_lengths, out, ids, empt
             bias_bs = bias.stride(0)
     if allowed is not None:
         states = allowed.shape[0]
-        if allowed.dim() != 2 or allowed.shape[1] != (V + 31) // 32 or states < 1 or allowed.dtype != torch.int32 or \
+        if allowed.dim() != 2 or allowed.shape[1] != (V + 31) // 32 or states < (B > 0) or allowed.dtype != torch.int32 or \
                 allowed.device != dev:
             raise ValueError("%s: allowed must be an int32 tensor [S, %d] on %s" % (who, (V + 31) // 32, dev))
         if not allowed.is_contiguous():
@@ -170,7 +170,7 @@ def control_logits(logits, control=None, history=None, lengths=None, prompt_leng
     ``history``: int32 / int64 tensor [B, T] of tokens so far, any strides (a [T, B] buffer's transpose is read in place);
     entries outside the vocabulary are passed over.  ``lengths``: integer tensor [B], how many of them count (default: all).
     ``prompt_lengths``: integer tensor [B], frequency and presence count from there on.  ``out``: where to write; ``logits``
-    itself changes them in place."""
+    itself changes them in place (memory that overlaps theirs in another way is refused)."""
     who = "control_logits"
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)

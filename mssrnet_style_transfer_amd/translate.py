@@ -18,6 +18,7 @@ def greedy_decode_cached(model, cfg, memory_bank, src_lengths, max_length, kv_bi
     TransformerDecoder.forward(step=s); finished sentences leave the batch at the check points.  Token ids int32 [steps, B],
     past a sentence's first </s> unspecified."""
     dev, B = memory_bank.device, memory_bank.size(1)
+    src_lengths = src_lengths.to(dev)
     lin = model.generator[0]
     with torch.no_grad():
         src = torch.zeros(memory_bank.size(0), B, 1, dtype=torch.long, device=dev)

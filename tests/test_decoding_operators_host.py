@@ -90,6 +90,21 @@ def test_token_control_refusals():
     assert lib.mssr_token_control_scratch(1, 20, 0) == 0 and lib.mssr_token_control_scratch(1, 100000, 0) > 0
 
 
+def test_new_logits_overlap_the_old_ones_in_place_or_not_at_all():
+    # rows of 50 fp32 words, 120 apart: their own place and other columns of the same rows hold nothing of another row.  A call
+    # without columns to spare that is let through would launch, so only refusals are made here.
+    for kw in (dict(out=FAKE + 4), dict(out=FAKE - 4), dict(out=FAKE + 4 * 49), dict(out=FAKE + 4 * 71, ld=120, ldo=120),
+               dict(out=FAKE + 4 * 49, ld=120, ldo=120), dict(out=FAKE - 4 * 71, ld=120, ldo=120),
+               dict(ld=120, ldo=110), dict(out=FAKE + 4 * 60, ld=120, ldo=110), dict(out=FAKE + 4 * 99)):
+        assert control(**kw) == 1, kw
+        assert b"overlap" in L.load().mssr_last_error(), kw
+    for kw in (dict(ids=FAKE, empty=1 << 31), dict(ids=FAKE, empty=-(1 << 31) - 1)):
+        assert control(**kw) == 1, kw
+        assert b"32-bit picks" in L.load().mssr_last_error(), kw
+    for kw in (dict(ld=1 << 40), dict(ldo=1 << 40)):
+        assert control(**kw) == 1, kw
+
+
 def test_pack_allowed():
     g = torch.Generator().manual_seed(3)
     for S, V in ((1, 1), (2, 32), (3, 33), (2, 95)):

@@ -418,3 +418,20 @@ def test_refusals(kv):
         c.write(x.cpu(), x.cpu())
     with torch.enable_grad(), pytest.raises(RuntimeError, match="no graph"):
         kv.attention(x.clone().requires_grad_(), c, 3)
+
+
+def test_data_that_moves_or_shrinks_in_place(kv):
+    k, q = heads(3, 2, 20, 64, torch.float32, 95), heads(3, 2, 1, 64, torch.float32, 96)
+    c = kv.KVCache4(3, 2, 64, 20)
+    c.write(k, k)
+    want = kv.attention(q, c, 20)
+    c.map(lambda t, dim: t[:2])                         # the same address, fewer sentences
+    assert c.batch == 2 and torch.equal(kv.attention(q[:2], c, 20), want[:2])
+    held = c.data
+    c.data = torch.cat([held, held])[2:]                # moved
+    held.zero_()
+    assert torch.equal(kv.attention(q[:2], c, 20), want[:2])
+    moved = c.data.clone()
+    c.data.set_(moved)                                  # the same tensor object, another address
+    c.write(k[:2] * 0, k[:2] * 0)
+    assert int(c.data.data_ptr()) == moved.data_ptr() and torch.equal(kv.attention(q[:2], c, 20), torch.zeros_like(want[:2]))

@@ -272,3 +272,40 @@ def test_refusals(tc):
             tc.pick_token(x, out=out)
     with pytest.raises(ValueError):
         tc.pack_allowed(words)
+
+
+def test_infinite_rates_leave_what_they_do_not_count(tc):
+    inf = float("inf")
+    x = torch.zeros(2, 40, device="cuda")
+    h = torch.tensor([[3, 5, 5, 7], [1, 1, 2, 3]], device="cuda")
+    first = torch.tensor([1, 2], device="cuda")
+    for c in (tc.TokenControl(frequency=inf), tc.TokenControl(presence=inf)):
+        got = tc.control_logits(x, c, h, prompt_lengths=first)
+        want = x.clone()
+        want[0, [5, 7]] = -inf                          # word 3 stands in the prompt only
+        want[1, [2, 3]] = -inf
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_where_the_new_logits_may_lie(tc, dtype):
+    g = torch.Generator(device="cuda").manual_seed(21)
+    both = torch.randn(5, 2 * 130 + 7, device="cuda", generator=g).to(dtype)
+    x, beside = both[:, :130], both[:, 137:]
+    c = tc.TokenControl(bias=torch.randn(130, device="cuda", generator=g))
+    want = tc.control_logits(x, c)
+    assert torch.equal(tc.control_logits(x, c, out=beside), want) and torch.equal(beside, want)
+    before = both.clone()
+    with pytest.raises(RuntimeError, match="overlap"):
+        tc.control_logits(x, c, out=both[:, 1:131])
+    with pytest.raises(RuntimeError, match="overlap"):
+        tc.control_logits(x[:4], c, out=both[1:, 3:133])
+    assert torch.equal(both, before)
+    assert torch.equal(tc.control_logits(x[:4], c, out=both[1:, 137:]), want[:4])       # other columns, a row further on
+    assert torch.equal(tc.control_logits(x, c, out=x), want) and torch.equal(x, want)
+
+
+def test_a_batch_without_rows(tc):
+    x = torch.zeros(0, 40, device="cuda")
+    each = tc.TokenControl(allowed=torch.zeros(0, 2, dtype=torch.int32, device="cuda"))
+    assert tc.control_logits(x, each).shape == (0, 40) and tc.pick_token(x, each).shape == (0,)
