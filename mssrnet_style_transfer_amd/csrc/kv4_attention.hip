@@ -91,6 +91,14 @@ __device__ __forceinline__ void kv4_pin(float& y) { asm volatile("" : "+v"(y)); 
 // the context cancel: rounded apart, an fp32 result of 1000 tokens was off by 1e-5)
 __device__ __forceinline__ float kv4_pow2(float x) { return __builtin_amdgcn_ldexpf(1.f, (int)fmaxf(x, -512.f)); }
 
+// The exponent of the power of two that bounds the V scales met so far; `top` becomes the largest fp16 number below it, so that
+// a larger scale alone, without a larger power of two, moves nothing.
+__device__ __forceinline__ int kv4_bound(float& top) {
+    const int e = __builtin_amdgcn_frexp_expf(top);
+    top = __builtin_amdgcn_ldexpf(1.f - 0x1p-11f, e);
+    return e;
+}
+
 // the product of this lane's quad, by two conditions (four nested ones become branches)
 __device__ __forceinline__ float kv4_own(float a, float b, float c, float d, bool odd, bool upper) {
     const float lo = odd ? b : a, hi = odd ? d : c;
@@ -357,7 +365,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
         }
         if (__any(far)) {
             vtop = fmaxf(vtop, wave_max(top));
-            const float e = vtop > 0.f ? (float)__builtin_amdgcn_frexp_expf(vtop) - KV4_UP : 0.f;
+            const float e = vtop > 0.f ? (float)kv4_bound(vtop) - KV4_UP : 0.f;
             f32x4 f = {1.f, 1.f, 1.f, 1.f};
 #pragma unroll
             for (int r = 0; r < R; ++r) {
@@ -548,7 +556,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
         for (int g = 0; g < NG; ++g) big = fmaxf(big, kv4_scale(mv[g]));
         if (__any(top > KV4_LAZY + KV4_UP || (fresh && top > -INFINITY) || big > vtop)) {
             vtop = fmaxf(vtop, wave_max(big));
-            const int e = vtop > 0.f ? __builtin_amdgcn_frexp_expf(vtop) : 0;
+            const int e = vtop > 0.f ? kv4_bound(vtop) : 0;
             const float shrink = __builtin_amdgcn_ldexpf(1.f, vexp - e);
             vexp = e;
             top = fmaxf(top, __shfl_xor(top, 16));
@@ -758,24 +766,26 @@ struct Kv4Shape { int rows, W, splits; int64_t units; };
 //   a wave each (W = 1) where units fill the chip: 4096 units of 140 tokens 12.5 against 18.7 with four waves; 2048 units
 //     of 1200 tokens 39.8 against 41.2, of more it evens out
 //   eight waves where units are few: 8 units of 1200 tokens 5.5 against 6.7 with four; 256 units of 5000 tokens 20 against
-//     25; but 512 units of 300 tokens 6.1 against 5.7, and many-row kernels on 512 units 10.9 against 8.0
+//     25; but 512 units of 300 tokens 6.1 against 5.7, and many-row kernels on 512 units 10.9 against 8.0.  4 rows: 256
+//     units of 2500 tokens 15.1 against 18.6, but 64 of 300 tokens 6.4 against 5.9
 //   splits, whose joining costs a second launch (3 us), where a unit's waves would go round more than four times and the
-//     chip has room: 8 units of 5000 tokens 7.2 against 11.3, 64 units (4 rows) of 8190 tokens 22 against 47; with 256
-//     units of 10000 tokens 42 against 38 unsplit.  128 units of 0 .. 32768 tokens: 8 splits 36, 2 splits 47.
+//     chip has room: 8 units of 5000 tokens 7.2 against 11.3; with 256 units of 10000 tokens 42 against 38 unsplit.  128
+//     units of 0 .. 32768 tokens: 8 splits 36, 2 splits 47.  4 rows, 64 units, as many splits as give 256 blocks: 8190
+//     tokens 17 against 27 (64 features), 32 against 61 (128, fp32); 1000 tokens 9.6 against 8.5 and 15.2 against 15.9
 static Kv4Shape kv4_shape(int64_t B, int Hkv, int NQ, int ng, int64_t longest) {
     Kv4Shape s;
     s.rows = NQ == 1 ? 1 : NQ <= 4 ? 4 : 16;
     s.units = B * Hkv * ((NQ + s.rows - 1) / s.rows);
     const int64_t nb = (longest + KV4_TOK - 1) / KV4_TOK;
     const bool crowd = s.units >= 2048 && nb <= 16;
-    const bool eight = s.rows != 4 && nb > 4 && (s.units <= 256 || (s.rows == 1 && nb >= 24));
+    const bool eight = s.rows == 4 ? nb >= 16 && s.units <= 256 : nb > 4 && (s.units <= 256 || (s.rows == 1 && nb >= 24));
     s.W = nb <= 1 || crowd ? 1 : eight ? 8 : 4;
     int64_t want = 1;
     if (s.rows == 1 && nb >= 36 && s.units <= 128) {
         const int64_t room = 1024 / s.units, use = nb / (8 * (1 + s.units / 64));
         want = room < use ? room : use;
     }
-    if (s.rows == 4 && nb >= 16 + s.units / 16) want = (ng <= 2 ? 512 : 256) / s.units;
+    if (s.rows == 4 && nb * ng >= 48 + s.units / 4) want = 256 / s.units;
     if (s.rows == 16 && nb >= 20) want = 256 / s.units;
     const int64_t most = (nb + s.W - 1) / s.W;
     s.splits = (int)(want < 1 ? 1 : (want > most ? most : want));
@@ -788,7 +798,7 @@ static void kv4_launch(const Kv4AttnArgs& a, const Kv4Shape& s, hipStream_t st) 
     const unsigned grid = W == 1 ? (a.units + 3) / 4 : a.units, threads = 64 * kv4_waves(W);
     if (s.rows == 1) kv4_few_kernel<T, NG, 1, W><<<grid, threads, 0, st>>>(a);
     else if (s.rows == 16) kv4_many_kernel<T, NG, W><<<grid, threads, 0, st>>>(a);
-    else if constexpr (W != 8) kv4_few_kernel<T, NG, 4, W><<<grid, threads, 0, st>>>(a);
+    else kv4_few_kernel<T, NG, 4, W><<<grid, threads, 0, st>>>(a);
 }
 template <typename T>
 static void kv4_dispatch(const Kv4AttnArgs& a, const Kv4Shape& s, int ng, hipStream_t st) {

@@ -435,3 +435,19 @@ def test_data_that_moves_or_shrinks_in_place(kv):
     c.data.set_(moved)                                  # the same tensor object, another address
     c.write(k[:2] * 0, k[:2] * 0)
     assert int(c.data.data_ptr()) == moved.data_ptr() and torch.equal(kv.attention(q[:2], c, 20), torch.zeros_like(want[:2]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,H,Hkv,dh,Tq,cap", [(2, 8, 2, 32, 1, 1100), (1, 12, 3, 96, 1, 1500), (3, 2, 2, 64, 1, 700),
+                                              (1, 4, 1, 128, 5, 1300)])
+def test_scales_that_grow_along_the_sentence(kv, dtype, B, H, Hkv, dh, Tq, cap):
+    # the V scales rise by 2^(1/5) a block, then jump up and down: within a power of two, past it, far past it
+    t = torch.arange(cap, device="cuda")
+    ramp = torch.exp2((t // 64) / 5.0) * torch.where(t % 300 == 299, 40.0, 1.0)
+    k, v = heads(B, Hkv, cap, dh, dtype, 61), (heads(B, Hkv, cap, dh, torch.float32, 62) * ramp[:, None]).to(dtype)
+    q = heads(B, H, Tq, dh, dtype, 63)
+    c = kv.KVCache4(B, Hkv, dh, cap)
+    c.write(k, v)
+    n = [cap - 3 * b for b in range(B)]
+    want, bound = attend(q, values(k), values(v), n, 1.0 / math.sqrt(dh), True)
+    close(kv.attention(q, c, torch.tensor(n, device="cuda"), causal=True), want, bound, "growing scales")
