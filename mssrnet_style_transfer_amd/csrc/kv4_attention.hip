@@ -25,9 +25,20 @@
 // sum is rescaled), so that a block of tokens costs one comparison and no cross-lane reduction.  The W waves of a block
 // take every W-th 64 tokens of its share of the sentence and are joined through LDS; a second launch joins the shares.
 #include "kv4.hpp"
-#include <type_traits>
 
 namespace mssr {
+
+// Division of a number below 2^31 by one the host knows: a high product, an addition, a shift
+// (m = floor(2^32 (2^shift - d) / d) + 1, shift = ceil(log2 d)).
+struct Divisor {
+    uint32_t d, m, shift;
+    Divisor() = default;
+    explicit Divisor(uint32_t n) : d(n), shift(0) {
+        while (((uint64_t)1 << shift) < n) ++shift;
+        m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - n)) / n + 1);
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return (__umulhi(m, x) + x) >> shift; }
+};
 
 struct Kv4AttnArgs {
     const uint8_t* data;
@@ -35,9 +46,10 @@ struct Kv4AttnArgs {
     const void* q;
     void* out;
     int64_t q_bs, q_hs, q_ts, o_bs, o_hs, o_ts;
-    int Hkv, G, Tq, dh, causal;     // G query heads share a key/value head
+    Divisor Hkv, Tq;
+    int G, dh, causal;              // G query heads share a key/value head
     int NQ;                         // G * Tq query rows of a (sentence, key/value head)
-    int splits;
+    Divisor splits, chunks;         // chunks of query rows
     IdxTable lengths;
     float scale;                    // of the scores, times log2(e)
     float* part;                    // [rows][splits][dh] unnormalised context, then [rows][splits][2] (max, sum)
@@ -130,20 +142,26 @@ constexpr int kv4_waves(int W) { return W == 1 ? 4 : W; }
 struct Kv4Work {            // what a block works on: query rows q0 .. of (sentence, key/value head), blocks [first, last)
     int64_t len;
     uint32_t b, bh;
-    int hk, q0, split, first, last;     // a sentence has fewer than 2^31 blocks (the entry point checks it)
+    int hk, q0, split, first, last;     // a sentence has at most 2^30 blocks (the entry point checks it)
     __device__ __forceinline__ Kv4Work(const Kv4AttnArgs& a, int rows, uint32_t id) {
-        split = id % (uint32_t)a.splits;
-        id /= (uint32_t)a.splits;
-        const uint32_t chunks = (uint32_t)(a.NQ + rows - 1) / (uint32_t)rows;
-        bh = id / chunks;
-        q0 = (int)(id - bh * chunks) * rows;
-        b = bh / (uint32_t)a.Hkv;
-        hk = (int)(bh - b * (uint32_t)a.Hkv);
+        const uint32_t unit = a.splits(id);
+        split = (int)(id - unit * a.splits.d);
+        bh = a.chunks(unit);
+        q0 = (int)(unit - bh * a.chunks.d) * rows;
+        b = a.Hkv(bh);
+        hk = (int)(bh - b * a.Hkv.d);
+    }
+    // query row k of the key/value head: new token i of head h (one row in all: ONE)
+    template <bool ONE>
+    __device__ __forceinline__ void row(const Kv4AttnArgs& a, int k, int& h, int& i) const {
+        const int u = ONE ? 0 : (int)a.Tq((uint32_t)k);
+        h = ONE ? hk : hk * a.G + u;
+        i = ONE ? 0 : k - u * (int)a.Tq.d;
     }
     __device__ __forceinline__ void span(const Kv4AttnArgs& a) {
         len = a.lengths.at(b);
         len = len < 0 ? 0 : (len > a.capacity ? a.capacity : len);
-        const uint32_t nb = (uint32_t)((len + KV4_TOK - 1) >> 6), per = (nb + (uint32_t)a.splits - 1) / (uint32_t)a.splits;
+        const uint32_t nb = (uint32_t)((len + KV4_TOK - 1) >> 6), per = a.splits(nb + a.splits.d - 1);
         const uint32_t lo = (uint32_t)split * per, hi = lo + per;
         first = (int)(lo < nb ? lo : nb);
         last = (int)(hi < nb ? hi : nb);
@@ -161,18 +179,15 @@ struct Kv4Query {
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             const int ch = g * 32 + quad * 8;
+            const bool in = have && ch < dh;     // the others read the row's first features and drop them
+            uint32_t raw[2 * sizeof(T)];
+            __builtin_memcpy(raw, src + (in ? ch : 0), sizeof(raw));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[g][e] = 0.f;
-            if (have && ch < dh) {
-                if constexpr (sizeof(T) == 4) {
-                    __builtin_memcpy(x[g], src + ch, 32);
-                } else {
-                    bf16x8 v;
-                    __builtin_memcpy(&v, src + ch, 16);
+            for (uint32_t& r : raw) r = in ? r : 0u;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[g][e] = (float)v[e];
-                }
-            }
+            for (int e = 0; e < 8; ++e)
+                x[g][e] = __builtin_bit_cast(float, sizeof(T) == 4 ? raw[e % (2 * sizeof(T))]
+                                                                   : e & 1 ? raw[e >> 1] & 0xffff0000u : raw[e >> 1] << 16);
 #pragma unroll
             for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[g][e]));
             float t = ((x[g][0] + x[g][1]) + (x[g][2] + x[g][3])) + ((x[g][4] + x[g][5]) + (x[g][6] + x[g][7]));
@@ -216,17 +231,19 @@ __device__ __forceinline__ void kv4_finish(const Kv4AttnArgs& a, const Kv4Work& 
             o0 = fmaf(f, om[k][r][c], o0);
             o1 = fmaf(f, om[k][r][c + 1], o1);
         }
-        if (a.splits == 1) {
-            const int i = qi % a.Tq, h = wk.hk * a.G + qi / a.Tq;
+        if (a.splits.d == 1) {
+            int h, i;
+            wk.template row<R == 1>(a, qi, h, i);
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
             T* dst = (T*)a.out + (int64_t)wk.b * a.o_bs + (int64_t)h * a.o_hs + (int64_t)i * a.o_ts + c;
-            dst[0] = from_f<T>(sum == 0.f ? 0.f : o0 / sum);
-            dst[1] = from_f<T>(sum == 0.f ? 0.f : o1 / sum);
+            dst[0] = from_f<T>(sum == 0.f ? 0.f : o0 * inv);
+            dst[1] = from_f<T>(sum == 0.f ? 0.f : o1 * inv);
         } else {
-            const int64_t at = ((int64_t)wk.bh * a.NQ + qi) * a.splits + wk.split;
+            const int64_t at = ((int64_t)wk.bh * a.NQ + qi) * a.splits.d + wk.split;
             a.part[at * a.dh + c] = o0;
             a.part[at * a.dh + c + 1] = o1;
             if (c == 0) {
-                float* ml = a.part + a.rows * a.splits * a.dh + at * 2;
+                float* ml = a.part + a.rows * a.splits.d * a.dh + at * 2;
                 ml[0] = top;
                 ml[1] = sum;
             }
@@ -257,10 +274,10 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
     Kv4Work wk(a, R, id);
     const uint8_t* base = a.data + (int64_t)wk.bh * a.blocks * kv4_block_bytes(NG);
     Kv4Tile<NG> cur;
-    const bool early = W == 1 && a.splits == 1;  // a lone wave's first block is known before its length is
+    const bool early = a.splits.d == 1 && w < a.blocks;      // an unsplit wave's first block is known before its length is
     if (early) {
-        cur.load_k(base, lane);
-        cur.load_v(base, lane);
+        cur.load_k(base + w * kv4_block_bytes(NG), lane);
+        cur.load_v(base + w * kv4_block_bytes(NG), lane);
     }
     wk.span(a);
     f16x8 qop[QROWS ? 1 : PARTS][NG];
@@ -269,14 +286,17 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
     {
         const int r = R == 1 ? 0 : (n & 3), qi = wk.q0 + r;
         const bool have = qi < a.NQ;
-        const int i = have ? qi % a.Tq : 0, h = wk.hk * a.G + (have ? qi / a.Tq : 0);
+        int h, i;
+        wk.template row<R == 1>(a, have ? qi : 0, h, i);
         Kv4Query<T, NG, PARTS> q;
         q.load((const T*)a.q + (int64_t)wk.b * a.q_bs + (int64_t)h * a.q_hs + (int64_t)i * a.q_ts, have, a.dh, quad);
         const float back = __builtin_amdgcn_ldexpf(a.scale, 24 - q.up);
 #pragma unroll
         for (int rr = 0; rr < R; ++rr) {
             const int k = wk.q0 + rr;
-            lim[rr] = k < a.NQ ? (a.causal ? wk.len - a.Tq + 1 + k % a.Tq : wk.len) : 0;
+            int hh, ii;
+            wk.template row<R == 1>(a, k, hh, ii);
+            lim[rr] = k < a.NQ ? (a.causal ? wk.len - (int)a.Tq.d + 1 + ii : wk.len) : 0;
             down[rr] = lane_read(back, rr);
 #pragma unroll
             for (int g = 0; g < NG; ++g) qsum[rr][g] = lane_read(q.sum[g], rr) * a.scale;
@@ -476,15 +496,24 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
     if (W == 1 && id >= a.units) return;
     auto& om = om_[W == 1 ? wave : 0];
     Kv4Work wk(a, 16, id);
+    const uint8_t* base = a.data + (int64_t)wk.bh * a.blocks * kv4_block_bytes(NG);
+    Kv4Tile<NG> cur;
+    const bool early = a.splits.d == 1 && w < a.blocks;
+    if (early) {
+        cur.load_k(base + w * kv4_block_bytes(NG), lane);
+        cur.load_v(base + w * kv4_block_bytes(NG), lane);
+    }
     wk.span(a);
     const int qi = wk.q0 + n;
     const bool have = qi < a.NQ;
-    const int64_t lim = have ? (a.causal ? wk.len - a.Tq + 1 + qi % a.Tq : wk.len) : 0;
-    // every row of the block sees at least this many tokens: blocks below it need no comparisons
-    const int64_t sure = wk.q0 + 16 > a.NQ ? 0 : a.causal ? wk.len - a.Tq + 1 : wk.len;
+    int h, i;
+    wk.template row<false>(a, have ? qi : 0, h, i);
+    const int64_t lim = have ? (a.causal ? wk.len - (int)a.Tq.d + 1 + i : wk.len) : 0;
+    // every row of the block sees at least this many tokens: blocks below it need no comparisons (rows that are not there
+    // may see anything)
+    const int64_t sure = a.causal ? wk.len - (int)a.Tq.d + 1 : wk.len;
     Kv4Query<T, NG, PARTS> q;
     {
-        const int i = have ? qi % a.Tq : 0, h = wk.hk * a.G + (have ? qi / a.Tq : 0);
         q.load((const T*)a.q + (int64_t)wk.b * a.q_bs + (int64_t)h * a.q_hs + (int64_t)i * a.q_ts, have, a.dh, quad);
     }
     // Q_g * 2^(up - 6) (below 2^13) in two parts: slots 0-3 and 4-7 of quad 0, against z_0..3 twice
@@ -508,14 +537,11 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
     for (int g = 0; g < (F32 ? NG : 1); ++g) zs[g] = 0.f;
 #pragma unroll
     for (int c = 0; c < 2 * NG; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const uint8_t* base = a.data + (int64_t)wk.bh * a.blocks * kv4_block_bytes(NG);
     const int col = (lane & 32) | ((lane & 12) << 1) | ((lane & 16) >> 2) | ((lane & 1) << 1) | ((lane >> 1) & 1);
     const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
     Token& my = tk[wave];
 
-    Kv4Tile<NG> cur;
-    auto step = [&](auto edge_c, int see, const uint32_t (&mv)[NG], const uint8_t* next) {
-        constexpr bool EDGE = decltype(edge_c)::value;
+    auto step = [&](bool edge, int see, const uint32_t (&mv)[NG], const uint8_t* next) {
         float s[4][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -542,7 +568,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
             __builtin_amdgcn_sched_barrier(0);   // a tile at a time: all at once would take the registers of a whole wave
         }
         if (next) cur.load_k(next, lane);
-        if (EDGE) {
+        if (edge) {
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -578,6 +604,10 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
                 for (int r = 0; r < 4; ++r) s[t][r] -= up;
         }
         const float vmul = __builtin_amdgcn_ldexpf(1.f, -vexp);
+        bool nan = false;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) nan |= kv4_scale(mv[g]) != kv4_scale(mv[g]);
+        const bool hidden = edge && __any(nan);  // a row may have a NaN scale that it does not see, and 0 times NaN is NaN
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             const float vz = kv4_zero(mv[g]);
@@ -636,7 +666,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
                         const int r = (j >> 1) | ((j & 1) << 1);
                         if (F32) zs[F32 ? g : 0] = fmaf(s[t][r], z4[r], zs[F32 ? g : 0]);
                         float y = s[t][r] * v4[r];
-                        if (EDGE) y = 16 * t + 4 * quad + r < see ? y : 0.f;            // a scale may be NaN
+                        if (__builtin_expect(hidden, 0)) y = 16 * t + 4 * quad + r < see ? y : 0.f;
                         if (F32) kv4_pin(y);
 #pragma unroll
                         for (int part = 0; part < PARTS; ++part) {
@@ -663,7 +693,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
     };
 
     const uint8_t* ahead = base + (int64_t)(wk.first + w) * kv4_block_bytes(NG);
-    if (wk.first + w < wk.last) {
+    if (!early && wk.first + w < wk.last) {
         cur.load_k(ahead, lane);
         cur.load_v(ahead, lane);
     }
@@ -683,12 +713,8 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
         }
         my.kz[lane] = make_uint2(z[0] | (z[1] << 16), z[2] | (z[3] << 16));
         __builtin_amdgcn_wave_barrier();
-        if ((int64_t)(blk + 1) * KV4_TOK > sure) {
-            const int64_t left = lim - at;
-            step(std::true_type{}, (int)(left > KV4_TOK ? KV4_TOK : left), mv, more ? ahead : nullptr);
-        } else {
-            step(std::false_type{}, KV4_TOK, mv, more ? ahead : nullptr);
-        }
+        const int64_t left = lim - at;
+        step((int64_t)(blk + 1) * KV4_TOK > sure, (int)(left > KV4_TOK ? KV4_TOK : left), mv, more ? ahead : nullptr);
         __builtin_amdgcn_wave_barrier();
         if (more) cur.load_v(ahead, lane);
     }
@@ -722,13 +748,13 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a) {
     __shared__ float fac[KV4_MAX_SPLITS], red[4][KV4_MAX_DH], sums[4];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t row = blockIdx.x;
-    const float2* ml = reinterpret_cast<const float2*>(a.part + a.rows * a.splits * a.dh) + row * a.splits;
-    const float* o = a.part + row * a.splits * a.dh;
+    const float2* ml = reinterpret_cast<const float2*>(a.part + a.rows * a.splits.d * a.dh) + row * a.splits.d;
+    const float* o = a.part + row * a.splits.d * a.dh;
     float top = -INFINITY;
-    for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, ml[s].x);      // every wave for itself
+    for (int s = lane; s < (int)a.splits.d; s += 64) top = fmaxf(top, ml[s].x);      // every wave for itself
     top = wave_max(top);
     float sum = 0.f;
-    for (int s = threadIdx.x; s < a.splits; s += 256) {
+    for (int s = threadIdx.x; s < (int)a.splits.d; s += 256) {
         const float2 x = ml[s];
         const float f = x.x == -INFINITY && x.y == 0.f ? 0.f : kv4_pow2(x.x - top);
         fac[s] = f;
@@ -742,7 +768,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a) {
     const int c = 2 * lane;
     if (c < a.dh) {
 #pragma unroll 4
-        for (int s = w; s < a.splits; s += 4) {
+        for (int s = w; s < (int)a.splits.d; s += 4) {
             const float2 x = *reinterpret_cast<const float2*>(o + (int64_t)s * a.dh + c);
             o0 = fmaf(fac[s], x.x, o0);
             o1 = fmaf(fac[s], x.y, o1);
@@ -753,9 +779,9 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a) {
     __syncthreads();
     if ((int)threadIdx.x >= a.dh) return;
     const float v = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
-    const int64_t bh = row / a.NQ;
-    const int qi = (int)(row % a.NQ), i = qi % a.Tq;
-    const int64_t b = bh / a.Hkv, h = (bh % a.Hkv) * a.G + qi / a.Tq;
+    // row = ((b, key/value head), head of its G, new token)
+    const uint32_t hi = a.Tq((uint32_t)row), i = (uint32_t)row - hi * a.Tq.d, bh = hi / (uint32_t)a.G, b = a.Hkv(bh);
+    const uint32_t h = (bh - b * a.Hkv.d) * a.G + (hi - bh * a.G);
     ((T*)a.out)[b * a.o_bs + h * a.o_hs + i * a.o_ts + threadIdx.x] = from_f<T>(sum == 0.f ? 0.f : v / sum);
 }
 
@@ -810,7 +836,7 @@ static void kv4_dispatch(const Kv4AttnArgs& a, const Kv4Shape& s, int ng, hipStr
         break;
     switch (ng) { MSSR_KV4_A(1) MSSR_KV4_A(2) MSSR_KV4_A(3) MSSR_KV4_A(4) }
 #undef MSSR_KV4_A
-    if (a.splits > 1) kv4_join_kernel<T><<<(unsigned)a.rows, 256, 0, st>>>(a);
+    if (a.splits.d > 1) kv4_join_kernel<T><<<(unsigned)a.rows, 256, 0, st>>>(a);
 }
 
 }  // namespace mssr
@@ -837,7 +863,7 @@ extern "C" int mssr_kv4_attention(const mssr_kv4_cache* c, const void* q, int64_
     MSSR_REQUIRE(mssr_kv4_bytes(c->B, c->H, c->capacity, c->dh) > 0 && aligned(c->data, 16),
                  "kv4_attention: cache of %lld x %d heads x %lld tokens x %d features (multiples of 8 up to %d)",
                  (long long)c->B, c->H, (long long)c->capacity, c->dh, KV4_MAX_DH);
-    MSSR_REQUIRE(c->capacity <= (int64_t)KV4_TOK * INT32_MAX, "kv4_attention: %lld tokens a sentence", (long long)c->capacity);
+    MSSR_REQUIRE(c->capacity <= (int64_t)KV4_TOK << 30, "kv4_attention: %lld tokens a sentence", (long long)c->capacity);
     MSSR_REQUIRE(valid_dtype(dtype), "kv4_attention: dtype %d", dtype);
     MSSR_REQUIRE(Tq >= 0 && H >= c->H && H % c->H == 0, "kv4_attention: %d query heads on %d, %lld rows", H, c->H, (long long)Tq);
     MSSR_REQUIRE(lengths || (length0 >= 0 && length0 <= c->capacity), "kv4_attention: length %lld of a cache of %lld",
@@ -852,8 +878,8 @@ extern "C" int mssr_kv4_attention(const mssr_kv4_cache* c, const void* q, int64_
     MSSR_REQUIRE(s.splits == 1 || (scratch && scratch_bytes >= rows * s.splits * (c->dh + 2) * (int64_t)sizeof(float)),
                  "kv4_attention: scratch of %lld bytes is too small", (long long)scratch_bytes);
     Kv4AttnArgs a{(const uint8_t*)c->data, (c->capacity + KV4_TOK - 1) / KV4_TOK, c->capacity, q, out, q_bs, q_hs, q_ts,
-                  o_bs, o_hs, o_ts, c->H, H / c->H, (int)Tq, c->dh, causal ? 1 : 0, NQ, s.splits,
-                  {lengths, lengths_are_64, length0}, scale * 1.4426950408889634f, (float*)scratch, rows, (uint32_t)(s.units * s.splits)};
+                  o_bs, o_hs, o_ts, Divisor(c->H), Divisor((uint32_t)Tq), H / c->H, c->dh, causal ? 1 : 0, NQ,
+                  Divisor(s.splits), Divisor((uint32_t)((NQ + s.rows - 1) / s.rows)), {lengths, lengths_are_64, length0}, scale * 1.4426950408889634f, (float*)scratch, rows, (uint32_t)(s.units * s.splits)};
     if (dtype == MSSR_F32) kv4_dispatch<float>(a, s, kv4_groups(c->dh), (hipStream_t)stream);
     else kv4_dispatch<bf16>(a, s, kv4_groups(c->dh), (hipStream_t)stream);
     MSSR_LAUNCH_OK("kv4_attention");
