@@ -123,15 +123,17 @@ template <int NG>
 struct Kv4Tile {
     u32x4 k[NG], v[NG];
     uint32_t mk[NG], mv[NG];
-    __device__ __forceinline__ void load_k(const uint8_t* blk, int lane) {
+    __device__ __forceinline__ void load_k(const uint8_t* blk, int lane, int64_t left = KV4_TOK) {
 #pragma unroll
-        for (int i = 0; i < NG; ++i) k[i] = *reinterpret_cast<const u32x4*>(blk + i * 1024 + lane * 16);
+        for (int i = 0; i < NG; ++i)
+            if (4 * i / NG < 2 || left > 32) k[i] = *reinterpret_cast<const u32x4*>(blk + i * 1024 + lane * 16);
         __builtin_memcpy(mk, __builtin_assume_aligned(blk + NG * 2048 + lane * (4 * NG), 4), 4 * NG);
     }
-    __device__ __forceinline__ void load_v(const uint8_t* blk, int lane) {
+    __device__ __forceinline__ void load_v(const uint8_t* blk, int lane, int64_t left = KV4_TOK) {
         __builtin_memcpy(mv, __builtin_assume_aligned(blk + NG * 2304 + lane * (4 * NG), 4), 4 * NG);
 #pragma unroll
-        for (int i = 0; i < NG; ++i) v[i] = *reinterpret_cast<const u32x4*>(blk + NG * 1024 + i * 1024 + lane * 16);
+        for (int i = 0; i < NG; ++i)
+            if (2 * i / NG < 1 || left > 32) v[i] = *reinterpret_cast<const u32x4*>(blk + NG * 1024 + i * 1024 + lane * 16);
     }
 };
 
@@ -370,7 +372,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
             }
             if (R > 1) __builtin_amdgcn_sched_barrier(0);        // a group at a time, for the registers
         }
-        if (more) cur.load_k(ahead, lane);
+        if (more) cur.load_k(ahead, lane, wk.len - at - W * KV4_TOK);
         float s[R];
         uint32_t mask[R];
         bool far = top > vtop;                   // NaN scales are passed over: they make their own features NaN and no others
@@ -440,7 +442,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
             acc[2 * g + 1] = F32 ? acc[2 * g + 1] + (c1 + mid) : c1;
         }
         __builtin_amdgcn_wave_barrier();
-        if (more) cur.load_v(ahead, lane);
+        if (more) cur.load_v(ahead, lane, wk.len - at - W * KV4_TOK);
     }
 
 #pragma unroll
