@@ -645,24 +645,46 @@ typedef struct {
 } mssr_kv4_cache;
 int64_t mssr_kv4_bytes(int64_t B, int H, int64_t capacity, int dh);     /* < 0: not a valid shape */
 
-/* Quantises tokens t < min(T, counts[b]) of k, v (element (b, h, t, c) at b*bs + h*hs + t*ts + c) to the positions
- * start[b] + t.  index_bits: 1 = start is int64, 2 = counts is int64. */
-int mssr_kv4_write(const mssr_kv4_cache* cache, const void* k, int64_t k_bs, int64_t k_hs, int64_t k_ts, const void* v,
-                   int64_t v_bs, int64_t v_hs, int64_t v_ts, int64_t T, const void* start, int64_t start0,
-                   const void* counts, int index_bits, int dtype, void* stream);
-/* The values that positions start[b] + t, t < min(T, counts[b]) stand for, rounded once to dtype; zero for the other t < T. */
-int mssr_kv4_read(const mssr_kv4_cache* cache, void* k, int64_t k_bs, int64_t k_hs, int64_t k_ts, void* v, int64_t v_bs,
-                  int64_t v_hs, int64_t v_ts, int64_t T, const void* start, int64_t start0, const void* counts,
-                  int index_bits, int dtype, void* stream);
+/* Tokens t < T of keys and values as they come: element (b, h, t, c) at b*bs + h*hs + t*ts + c, at the cache's positions
+ * start[b] + t. */
+typedef struct {
+    const mssr_kv4_cache* cache;
+    void* k;                      /* [B, H, T, dh] of dtype: read by mssr_kv4_write, written by mssr_kv4_read */
+    int64_t k_bs, k_hs, k_ts;
+    void* v;
+    int64_t v_bs, v_hs, v_ts;
+    int64_t T;
+    const void* start;            /* [B], or NULL: start0 */
+    int64_t start0;
+    const void* counts;           /* [B], or NULL: T */
+    int index_bits;               /* 64-bit: 1 start, 2 counts */
+    int dtype;
+} mssr_kv4_rows;
+/* Quantises the tokens t < min(T, counts[b]) of k, v. */
+int mssr_kv4_write(const mssr_kv4_rows* rows, void* stream);
+/* The values that those positions stand for, rounded once to dtype; zero for the other t < T. */
+int mssr_kv4_read(const mssr_kv4_rows* rows, void* stream);
 /* out = softmax(scale * q k^T) v of Tq query rows over the first lengths[b] cached tokens (causal: row i over the first
  * lengths[b] - Tq + 1 + i); a row that sees no token gives zeros.  H query heads, a multiple of the cache's: head h reads
  * key/value head h / (H / cache->H).  `longest`: an upper bound of the lengths if the caller knows one (0: the capacity);
  * it only shapes the launch.  scratch: mssr_kv4_attention_scratch() bytes, free again when the call's work is done. */
+typedef struct {
+    const mssr_kv4_cache* cache;
+    const void* q;                /* [B, H, Tq, dh] of dtype, strides as above */
+    int64_t q_bs, q_hs, q_ts;
+    void* out;                    /* the same shape */
+    int64_t o_bs, o_hs, o_ts;
+    int64_t Tq;
+    const void* lengths;          /* [B], or NULL: length0 */
+    int64_t length0, longest;
+    void* scratch;
+    int64_t scratch_bytes;
+    int H, lengths_are_64;
+    float scale;
+    int causal, dtype;
+} mssr_kv4_attention_desc;
 int64_t mssr_kv4_attention_scratch(const mssr_kv4_cache* cache, int64_t Tq, int H, int64_t longest, int dtype);
-int mssr_kv4_attention(const mssr_kv4_cache* cache, const void* q, int64_t q_bs, int64_t q_hs, int64_t q_ts, void* out,
-                       int64_t o_bs, int64_t o_hs, int64_t o_ts, int H, int64_t Tq, const void* lengths, int64_t length0,
-                       int lengths_are_64, int64_t longest, float scale, int causal, void* scratch, int64_t scratch_bytes,
-                       int dtype, void* stream);
+int mssr_kv4_attention(const mssr_kv4_attention_desc* desc, void* stream);
 
 /* --------------------------------------------------------- control of the next token's logits --
  * What a decoding step does to its logits before it picks (the search of onmt/translate/greedy_search.py:135-165 and the

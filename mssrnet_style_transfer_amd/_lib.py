@@ -5,6 +5,7 @@ fallback: if the shared object is missing or a call fails, a RuntimeError is rai
 """
 import ctypes
 import os
+import struct
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int64, c_uint64, c_void_p
 
 import torch
@@ -100,6 +101,22 @@ class Kv4Cache(Structure):
     _fields_ = [("data", c_void_p), ("B", c_int64), ("capacity", c_int64), ("H", c_int), ("dh", c_int)]
 
 
+class Kv4Rows(Structure):
+    """mssr_kv4_rows (include/mssr_hip.h)."""
+    _fields_ = [("cache", c_void_p), ("k", c_void_p), ("k_bs", c_int64), ("k_hs", c_int64), ("k_ts", c_int64), ("v", c_void_p),
+                ("v_bs", c_int64), ("v_hs", c_int64), ("v_ts", c_int64), ("T", c_int64), ("start", c_void_p),
+                ("start0", c_int64), ("counts", c_void_p), ("index_bits", c_int), ("dtype", c_int)]
+
+
+class Kv4AttentionDesc(Structure):
+    """mssr_kv4_attention_desc (include/mssr_hip.h)."""
+    _fields_ = [("cache", c_void_p), ("q", c_void_p), ("q_bs", c_int64), ("q_hs", c_int64), ("q_ts", c_int64),
+                ("out", c_void_p), ("o_bs", c_int64), ("o_hs", c_int64), ("o_ts", c_int64), ("Tq", c_int64),
+                ("lengths", c_void_p), ("length0", c_int64), ("longest", c_int64), ("scratch", c_void_p),
+                ("scratch_bytes", c_int64), ("H", c_int), ("lengths_are_64", c_int), ("scale", c_float), ("causal", c_int),
+                ("dtype", c_int)]
+
+
 class TokenControlDesc(Structure):
     """mssr_token_control_desc (include/mssr_hip.h)."""
     _fields_ = [("logits", c_void_p), ("out", c_void_p), ("B", c_int64), ("V", c_int64), ("ld", c_int64), ("ldo", c_int64),
@@ -109,6 +126,15 @@ class TokenControlDesc(Structure):
                 ("bias", c_void_p), ("bias_bs", c_int64), ("allowed", c_void_p), ("states", c_int64), ("state", c_void_p),
                 ("state_mode", c_int), ("ids", c_void_p), ("empty", c_int64), ("index_bits", c_int), ("dtype", c_int),
                 ("scratch", c_void_p), ("scratch_bytes", c_int64)]
+
+
+_CODES = {c_void_p: "P", c_int64: "q", c_int: "i", c_float: "f"}
+
+
+def packer(desc):
+    """pack(*fields) of a descriptor: its bytes, which the C entry points take in its place.  For the calls of a decoding
+    step, where the host counts: a call of 24 arguments is 3.0 us, one of packed bytes 0.8 (a null pointer is 0 here)."""
+    return struct.Struct("@" + "".join(_CODES[t] for _, t in desc._fields_) + "0P").pack
 
 
 class PackJob(Structure):
@@ -185,13 +211,12 @@ SIGNATURES = {
     "mssr_decode_graphs_recorded": ([], ctypes.c_long),
     "mssr_decode_graphs_enable": ([_I], c_int),
     "mssr_kv4_bytes": ([_L, _I, _L, _I], c_int64),
-    "mssr_kv4_write": ([POINTER(Kv4Cache), _P, _L, _L, _L, _P, _L, _L, _L, _L, _P, _L, _P, _I, _I, _P], c_int),
-    "mssr_kv4_read": ([POINTER(Kv4Cache), _P, _L, _L, _L, _P, _L, _L, _L, _L, _P, _L, _P, _I, _I, _P], c_int),
+    "mssr_kv4_write": ([_P, _P], c_int),                       # the descriptor of these and the next ones: packer()
+    "mssr_kv4_read": ([_P, _P], c_int),
     "mssr_kv4_attention_scratch": ([POINTER(Kv4Cache), _L, _I, _L, _I], c_int64),
-    "mssr_kv4_attention": ([POINTER(Kv4Cache), _P, _L, _L, _L, _P, _L, _L, _L, _I, _L, _P, _L, _I, _L, _F, _I, _P, _L, _I, _P],
-                           c_int),
+    "mssr_kv4_attention": ([_P, _P], c_int),
     "mssr_token_control_scratch": ([_L, _L, _L], c_int64),
-    "mssr_token_control": ([POINTER(TokenControlDesc), _P], c_int),
+    "mssr_token_control": ([_P, _P], c_int),
     "mssr_debug_stamps": ([_P], None),
     "mssr_ctx_kv_grad": ([_P, _P, _L, _P, _L, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P], c_int),
 }
@@ -222,6 +247,19 @@ def check(rc, what=""):
     if rc != 0:
         msg = load().mssr_last_error().decode("utf-8", "replace")
         raise RuntimeError("libmssr_hip %s failed (code %d): %s" % (what, rc, msg))
+
+
+def call(name, device, desc):
+    """One C call ``name(desc, stream)`` on the device's current stream; a device that is not current becomes it meanwhile."""
+    index = device.index
+    fn = getattr(load(), name)
+    if index == torch.cuda.current_device():
+        rc = fn(desc, raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(desc, raw_stream(index))
+    if rc != 0:
+        check(rc, name)
 
 
 def dt(t):

@@ -857,31 +857,34 @@ extern "C" int64_t mssr_kv4_attention_scratch(const mssr_kv4_cache* c, int64_t T
     return s.splits > 1 ? c->B * c->H * NQ * s.splits * (c->dh + 2) * (int64_t)sizeof(float) : 0;
 }
 
-extern "C" int mssr_kv4_attention(const mssr_kv4_cache* c, const void* q, int64_t q_bs, int64_t q_hs, int64_t q_ts, void* out,
-                                  int64_t o_bs, int64_t o_hs, int64_t o_ts, int H, int64_t Tq, const void* lengths,
-                                  int64_t length0, int lengths_are_64, int64_t longest, float scale, int causal, void* scratch,
-                                  int64_t scratch_bytes, int dtype, void* stream) {
-    MSSR_REQUIRE(c && c->data && (Tq == 0 || (q && out)), "kv4_attention: null operand");
+extern "C" int mssr_kv4_attention(const mssr_kv4_attention_desc* d, void* stream) {
+    MSSR_REQUIRE(d && d->cache, "kv4_attention: null operand");
+    const mssr_kv4_cache* c = d->cache;
+    const int H = d->H, dtype = d->dtype;
+    const int64_t Tq = d->Tq;
+    MSSR_REQUIRE(c->data && (Tq == 0 || (d->q && d->out)), "kv4_attention: null operand");
     MSSR_REQUIRE(mssr_kv4_bytes(c->B, c->H, c->capacity, c->dh) > 0 && aligned(c->data, 16),
                  "kv4_attention: cache of %lld x %d heads x %lld tokens x %d features (multiples of 8 up to %d)",
                  (long long)c->B, c->H, (long long)c->capacity, c->dh, KV4_MAX_DH);
     MSSR_REQUIRE(c->capacity <= (int64_t)KV4_TOK << 30, "kv4_attention: %lld tokens a sentence", (long long)c->capacity);
     MSSR_REQUIRE(valid_dtype(dtype), "kv4_attention: dtype %d", dtype);
     MSSR_REQUIRE(Tq >= 0 && H >= c->H && H % c->H == 0, "kv4_attention: %d query heads on %d, %lld rows", H, c->H, (long long)Tq);
-    MSSR_REQUIRE(lengths || (length0 >= 0 && length0 <= c->capacity), "kv4_attention: length %lld of a cache of %lld",
-                 (long long)length0, (long long)c->capacity);
+    MSSR_REQUIRE(d->lengths || (d->length0 >= 0 && d->length0 <= c->capacity), "kv4_attention: length %lld of a cache of %lld",
+                 (long long)d->length0, (long long)c->capacity);
     if (Tq == 0) return MSSR_OK;
     MSSR_REQUIRE(Tq <= (INT32_MAX >> 8) / (H / c->H), "kv4_attention: %lld query rows", (long long)Tq);
     const int NQ = (int)(H / c->H * Tq);
-    const Kv4Shape s = kv4_shape(c->B, c->H, NQ, kv4_groups(c->dh), kv4_longest(c, longest));
+    const Kv4Shape s = kv4_shape(c->B, c->H, NQ, kv4_groups(c->dh), kv4_longest(c, d->longest));
     const int64_t rows = c->B * c->H * NQ;
     MSSR_REQUIRE(s.units <= KV4_MAX_GRID / s.splits && rows <= KV4_MAX_GRID, "kv4_attention: %lld query rows in one call",
                  (long long)rows);
-    MSSR_REQUIRE(s.splits == 1 || (scratch && scratch_bytes >= rows * s.splits * (c->dh + 2) * (int64_t)sizeof(float)),
-                 "kv4_attention: scratch of %lld bytes is too small", (long long)scratch_bytes);
-    Kv4AttnArgs a{(const uint8_t*)c->data, (c->capacity + KV4_TOK - 1) / KV4_TOK, c->capacity, q, out, q_bs, q_hs, q_ts,
-                  o_bs, o_hs, o_ts, Divisor(c->H), Divisor((uint32_t)Tq), H / c->H, c->dh, causal ? 1 : 0, NQ,
-                  Divisor(s.splits), Divisor((uint32_t)((NQ + s.rows - 1) / s.rows)), {lengths, lengths_are_64, length0}, scale * 1.4426950408889634f, (float*)scratch, rows, (uint32_t)(s.units * s.splits)};
+    MSSR_REQUIRE(s.splits == 1 || (d->scratch && d->scratch_bytes >= rows * s.splits * (c->dh + 2) * (int64_t)sizeof(float)),
+                 "kv4_attention: scratch of %lld bytes is too small", (long long)d->scratch_bytes);
+    Kv4AttnArgs a{(const uint8_t*)c->data, (c->capacity + KV4_TOK - 1) / KV4_TOK, c->capacity, d->q, d->out,
+                  d->q_bs, d->q_hs, d->q_ts, d->o_bs, d->o_hs, d->o_ts, Divisor(c->H), Divisor((uint32_t)Tq), H / c->H,
+                  c->dh, d->causal ? 1 : 0, NQ, Divisor(s.splits), Divisor((uint32_t)((NQ + s.rows - 1) / s.rows)),
+                  {d->lengths, d->lengths_are_64, d->length0}, d->scale * 1.4426950408889634f, (float*)d->scratch, rows,
+                  (uint32_t)(s.units * s.splits)};
     if (dtype == MSSR_F32) kv4_dispatch<float>(a, s, kv4_groups(c->dh), (hipStream_t)stream);
     else kv4_dispatch<bf16>(a, s, kv4_groups(c->dh), (hipStream_t)stream);
     MSSR_LAUNCH_OK("kv4_attention");

@@ -327,6 +327,19 @@ static int kv4_check(const mssr_kv4_cache* c, const char* who) {
     MSSR_REQUIRE(aligned(c->data, 16), "%s: the cache must be 16-byte aligned", who);
     return MSSR_OK;
 }
+static int kv4_check_rows(const mssr_kv4_rows* r, const char* who) {
+    MSSR_REQUIRE(r, "%s: no descriptor", who);
+    if (int rc = kv4_check(r->cache, who)) return rc;
+    MSSR_REQUIRE(r->T == 0 || (r->k && r->v), "%s: null keys or values", who);
+    MSSR_REQUIRE(valid_dtype(r->dtype), "%s: dtype %d", who, r->dtype);
+    MSSR_REQUIRE(r->T >= 0, "%s: %lld tokens", who, (long long)r->T);
+    MSSR_REQUIRE((r->index_bits & ~3) == 0, "%s: index_bits %d", who, r->index_bits);
+    const int64_t capacity = r->cache->capacity;
+    MSSR_REQUIRE(r->start || (r->start0 >= 0 && r->T <= capacity && r->start0 <= capacity - r->T),
+                 "%s: %lld tokens from %lld on in a cache of %lld", who, (long long)r->T, (long long)r->start0,
+                 (long long)capacity);
+    return MSSR_OK;
+}
 static Kv4View kv4_view(const mssr_kv4_cache* c) {
     return Kv4View{(uint8_t*)c->data, (c->capacity + KV4_TOK - 1) / KV4_TOK, c->capacity, c->H, c->dh};
 }
@@ -346,22 +359,16 @@ extern "C" int64_t mssr_kv4_bytes(int64_t B, int H, int64_t capacity, int dh) {
 // tokens a sentence from which a call collects whole blocks in LDS
 static constexpr int64_t KV4_BLOCK_MIN_T = 16;
 
-extern "C" int mssr_kv4_write(const mssr_kv4_cache* c, const void* k, int64_t k_bs, int64_t k_hs, int64_t k_ts, const void* v,
-                              int64_t v_bs, int64_t v_hs, int64_t v_ts, int64_t T, const void* start, int64_t start0,
-                              const void* counts, int index_bits, int dtype, void* stream) {
-    if (int rc = kv4_check(c, "kv4_write")) return rc;
-    MSSR_REQUIRE(T == 0 || (k && v), "kv4_write: null keys or values");
-    MSSR_REQUIRE(valid_dtype(dtype), "kv4_write: dtype %d", dtype);
-    MSSR_REQUIRE(T >= 0, "kv4_write: %lld tokens", (long long)T);
-    MSSR_REQUIRE((index_bits & ~3) == 0, "kv4_write: index_bits %d", index_bits);
-    MSSR_REQUIRE(start || (start0 >= 0 && T <= c->capacity && start0 <= c->capacity - T),
-                 "kv4_write: tokens %lld .. %lld of a cache of %lld", (long long)start0, (long long)(start0 + T),
-                 (long long)c->capacity);
+extern "C" int mssr_kv4_write(const mssr_kv4_rows* r, void* stream) {
+    if (int rc = kv4_check_rows(r, "kv4_write")) return rc;
+    const mssr_kv4_cache* c = r->cache;
+    const int64_t T = r->T;
+    const int dtype = r->dtype;
     if (T == 0) return MSSR_OK;
     const int ng = kv4_groups(c->dh);
     hipStream_t s = (hipStream_t)stream;
-    Kv4WriteArgs a{kv4_view(c), k, v, k_bs, k_hs, k_ts, v_bs, v_hs, v_ts, T, {start, index_bits & 1, start0},
-                   {counts, (index_bits >> 1) & 1, 0}, 0};
+    Kv4WriteArgs a{kv4_view(c), r->k, r->v, r->k_bs, r->k_hs, r->k_ts, r->v_bs, r->v_hs, r->v_ts, T,
+                  {r->start, r->index_bits & 1, r->start0}, {r->counts, (r->index_bits >> 1) & 1, 0}, 0};
     const int64_t bh = c->B * c->H;
     if (T < KV4_BLOCK_MIN_T && bh <= (int64_t)1 << 27 && bh * T * ng * 4 < (int64_t)1 << 31) {
         a.items = bh * T * ng * 4;
@@ -384,22 +391,16 @@ extern "C" int mssr_kv4_write(const mssr_kv4_cache* c, const void* k, int64_t k_
     MSSR_LAUNCH_OK("kv4_write");
 }
 
-extern "C" int mssr_kv4_read(const mssr_kv4_cache* c, void* k, int64_t k_bs, int64_t k_hs, int64_t k_ts, void* v, int64_t v_bs,
-                             int64_t v_hs, int64_t v_ts, int64_t T, const void* start, int64_t start0, const void* counts,
-                             int index_bits, int dtype, void* stream) {
-    if (int rc = kv4_check(c, "kv4_read")) return rc;
-    MSSR_REQUIRE(T == 0 || (k && v), "kv4_read: null keys or values");
-    MSSR_REQUIRE(valid_dtype(dtype), "kv4_read: dtype %d", dtype);
-    MSSR_REQUIRE(T >= 0, "kv4_read: %lld tokens", (long long)T);
-    MSSR_REQUIRE((index_bits & ~3) == 0, "kv4_read: index_bits %d", index_bits);
-    MSSR_REQUIRE(start || (start0 >= 0 && T <= c->capacity && start0 <= c->capacity - T),
-                 "kv4_read: tokens %lld .. %lld of a cache of %lld", (long long)start0, (long long)(start0 + T),
-                 (long long)c->capacity);
+extern "C" int mssr_kv4_read(const mssr_kv4_rows* r, void* stream) {
+    if (int rc = kv4_check_rows(r, "kv4_read")) return rc;
+    const mssr_kv4_cache* c = r->cache;
+    const int64_t T = r->T;
+    const int dtype = r->dtype;
     if (T == 0) return MSSR_OK;
     const int ng = kv4_groups(c->dh);
     hipStream_t s = (hipStream_t)stream;
-    Kv4ReadArgs a{kv4_view(c), k, v, k_bs, k_hs, k_ts, v_bs, v_hs, v_ts, T, {start, index_bits & 1, start0},
-                  {counts, (index_bits >> 1) & 1, 0}, 0};
+    Kv4ReadArgs a{kv4_view(c), r->k, r->v, r->k_bs, r->k_hs, r->k_ts, r->v_bs, r->v_hs, r->v_ts, T,
+                  {r->start, r->index_bits & 1, r->start0}, {r->counts, (r->index_bits >> 1) & 1, 0}, 0};
     const int64_t bh = c->B * c->H;
     if (T < KV4_BLOCK_MIN_T && bh <= (int64_t)1 << 27 && bh * T * ng * 4 < (int64_t)1 << 31) {
         a.items = bh * T * ng * 4;

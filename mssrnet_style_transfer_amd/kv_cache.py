@@ -8,6 +8,7 @@ reference keeps 32.  Tokens are quantised once, when they are written; ``attenti
 These are decoding operators: they build no graph and refuse inputs that would need one.
 """
 import ctypes
+from functools import lru_cache
 
 import torch
 
@@ -17,6 +18,7 @@ MAX_DIM = 128
 
 
 _INTS = (torch.int32, torch.int64)
+_pack_rows, _pack_attention = L.packer(L.Kv4Rows), L.packer(L.Kv4AttentionDesc)
 
 
 def _needs_graph(who):
@@ -34,12 +36,14 @@ def _index(who, name, t, B, device):
     return (t if t.is_contiguous() else t.contiguous()), 0, int(dtype is torch.int64)
 
 
-def _launch(device, fn, *args):
-    """fn(*args, stream) on the device's current stream; the device is made current for the call where it is not."""
-    if device.index == torch.cuda.current_device():
-        return fn(*args, L.raw_stream(device.index))
-    with torch.cuda.device(device):
-        return fn(*args, L.raw_stream(device.index))
+def _address(t):
+    return 0 if t is None else t.data_ptr()
+
+
+@lru_cache(maxsize=1024)
+def _scratch_bytes(B, Hkv, capacity, dh, T, H, longest, code):
+    """How much scratch a shape takes: a number of the shape alone."""
+    return L.load().mssr_kv4_attention_scratch(ctypes.byref(L.Kv4Cache(None, B, capacity, Hkv, dh)), T, H, longest, code)
 
 
 class KVCache4:
@@ -75,11 +79,11 @@ class KVCache4:
         return dict(self.__dict__, _held=None)      # checkpoints and copies hold the data, not its address
 
     def _desc(self):
-        """byref of the C descriptor of the present data (built again where that has moved or changed its batch)."""
+        """The address of the C descriptor of the present data (built again where that has moved or changed its batch)."""
         at = (self.data.data_ptr(), self.data.shape[0])
         if self._held is None or self._held[0] != at:
             d = L.Kv4Cache(*at, self.capacity, self.heads, self.dim)
-            self._held = (at, d, ctypes.byref(d))
+            self._held = (at, d, ctypes.addressof(d))
         return self._held[2]
 
     def _span(self, who, start, T, counts):
@@ -123,8 +127,9 @@ class KVCache4:
             return
         kb, kh, kt, _ = k.stride()
         vb, vh, vt, _ = v.stride()
-        L.check(_launch(device, L.load().mssr_kv4_write, self._desc(), k.data_ptr(), kb, kh, kt, v.data_ptr(), vb, vh, vt, T,
-                        L.ptr(start), start0, L.ptr(counts), bits, L.dt(k)), "kv4_write")
+        L.call("mssr_kv4_write", device, _pack_rows(
+            self._desc(), k.data_ptr(), kb, kh, kt, v.data_ptr(), vb, vh, vt, T, _address(start), start0, _address(counts),
+            bits, L.dt(k)))
 
     def read(self, start, length, counts=None, dtype=torch.float32):
         """(k, v), each [B, heads, length, dim] (a view of [B, length, heads, dim] memory), of positions ``start`` + 0 ..
@@ -140,8 +145,9 @@ class KVCache4:
         k, v = both.unbind(0)
         if B == 0:
             return k, v
-        L.check(_launch(self.device, L.load().mssr_kv4_read, self._desc(), k.data_ptr(), T * H * dh, dh, H * dh, v.data_ptr(),
-                        T * H * dh, dh, H * dh, T, L.ptr(start), start0, L.ptr(counts), bits, L.dt(k)), "kv4_read")
+        L.call("mssr_kv4_read", self.device, _pack_rows(
+            self._desc(), k.data_ptr(), T * H * dh, dh, H * dh, v.data_ptr(), T * H * dh, dh, H * dh, T, _address(start),
+            start0, _address(counts), bits, L.dt(k)))
         return k, v
 
     def map(self, fn):
@@ -180,12 +186,11 @@ def attention(q, cache, lengths, scale=None, causal=False, longest=0):
     out = torch.empty_strided((B, H, T, dh), (T * H * dh, dh, H * dh, 1), dtype=q.dtype, device=device)
     if T == 0 or B == 0:
         return out
-    lib, d = L.load(), cache._desc()
-    need = lib.mssr_kv4_attention_scratch(d, T, H, longest, code)
+    need = _scratch_bytes(B, cache.heads, cache.capacity, dh, T, H, longest, code)
     # from the allocator, per call: a call's scratch is its own on every stream and in every captured graph
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
     qb, qh, qt, _ = q.stride()
-    L.check(_launch(device, lib.mssr_kv4_attention, d, q.data_ptr(), qb, qh, qt, out.data_ptr(), T * H * dh, dh, H * dh, H, T,
-                    L.ptr(lengths), n, wide, longest, dh ** -0.5 if scale is None else scale, 1 if causal else 0, L.ptr(ws),
-                    need, code), "kv4_attention")
+    L.call("mssr_kv4_attention", device, _pack_attention(
+        cache._desc(), q.data_ptr(), qb, qh, qt, out.data_ptr(), T * H * dh, dh, H * dh, T, _address(lengths), n, longest,
+        _address(ws), need, H, wide, dh ** -0.5 if scale is None else scale, 1 if causal else 0, code))
     return out

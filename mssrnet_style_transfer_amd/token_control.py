@@ -4,8 +4,8 @@ What stands between a decoder's generator and its pick (the reference's search t
 onmt/translate/greedy_search.py:135-165, with its n-gram rule in onmt/translate/decode_strategy.py): one pass over the
 logits, which leaves either new logits (for a sampler) or only the picked ids.  Decoding operators: they build no graph.
 """
-import ctypes
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import Optional, Union
 
 import torch
@@ -60,6 +60,13 @@ def pack_allowed(allowed):
 
 
 _INTS = (torch.int32, torch.int64)
+_pack = L.packer(L.TokenControlDesc)
+
+
+@lru_cache(maxsize=1024)
+def _scratch_bytes(B, V, T):
+    """How much scratch a pick of this shape takes: a number of the shape alone."""
+    return L.load().mssr_token_control_scratch(B, V, T)
 
 
 def _int_error(who, name, shape, device):
@@ -81,6 +88,10 @@ def _rate(who, name, x, B, device):
         raise ValueError("%s: %s must be a number or a float32 tensor [%d] on %s (got %s %s on %s)" % (
             who, name, B, device, x.dtype, tuple(x.shape), x.device))
     return (x if x.is_contiguous() else x.contiguous()), 0.0
+
+
+def _address(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _call(who, logits, control, history, lengths, prompt_lengths, out, ids, empty):
@@ -146,22 +157,18 @@ def _call(who, logits, control, history, lengths, prompt_lengths, out, ids, empt
     code = L.dt(logits)
     if B == 0:
         return
-    lib, ptr, ws, need = L.load(), L.ptr, None, 0
+    ws, need = None, 0
     if ids is not None:
         bits |= 16 * int(ids.dtype is torch.int64)
-        need = lib.mssr_token_control_scratch(B, V, T)
+        need = _scratch_bytes(B, V, T)
         if need > 0:                             # a call's own: streams and captured graphs share none
             ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    d = L.TokenControlDesc(logits.data_ptr(), ptr(out), B, V, logits.stride(0) if B > 1 else V,
-                           0 if out is None else (out.stride(0) if B > 1 else V), ptr(history), h_bs, h_ts, T, ptr(lengths),
-                           ptr(prompt_lengths), ptr(rep), ptr(freq), ptr(pres), rep0, freq0, pres0, int(c.ngram), ptr(bias),
-                           bias_bs, ptr(allowed), states, ptr(state), mode, ptr(ids), int(empty), bits, code, ptr(ws), need)
-    if dev.index == torch.cuda.current_device():
-        rc = lib.mssr_token_control(ctypes.byref(d), L.raw_stream(dev.index))
-    else:
-        with torch.cuda.device(dev):
-            rc = lib.mssr_token_control(ctypes.byref(d), L.raw_stream(dev.index))
-    L.check(rc, "token_control")
+    ptr = _address
+    L.call("mssr_token_control", dev, _pack(
+        logits.data_ptr(), ptr(out), B, V, logits.stride(0) if B > 1 else V,
+        0 if out is None else (out.stride(0) if B > 1 else V), ptr(history), h_bs, h_ts, T, ptr(lengths),
+        ptr(prompt_lengths), ptr(rep), ptr(freq), ptr(pres), rep0, freq0, pres0, int(c.ngram), ptr(bias), bias_bs, ptr(allowed),
+        states, ptr(state), mode, ptr(ids), int(empty), bits, code, ptr(ws), need))
 
 
 def control_logits(logits, control=None, history=None, lengths=None, prompt_lengths=None, out=None):

@@ -30,7 +30,8 @@ def test_cache_refusals(fn):
     lib = L.load()
 
     def call(c, k=FAKE, v=FAKE, T=3, start=None, start0=0, counts=None, bits=0, dtype=L.F32):
-        return getattr(lib, fn)(ctypes.byref(c), k, 0, 0, 64, v, 0, 0, 64, T, start, start0, counts, bits, dtype, None)
+        r = L.Kv4Rows(ctypes.addressof(c), k, 0, 0, 64, v, 0, 0, 64, T, start, start0, counts, bits, dtype)
+        return getattr(lib, fn)(ctypes.byref(r), None)
 
     for c in (cache(data=None), cache(dh=60), cache(dh=0), cache(dh=256), cache(B=0), cache(H=0), cache(capacity=0),
               cache(data=FAKE + 8)):
@@ -48,8 +49,9 @@ def test_attention_refusals():
     lib = L.load()
 
     def call(c, q=FAKE, out=FAKE, H=2, Tq=1, lengths=None, n=10, longest=0, scratch=None, nbytes=0, dtype=L.F32):
-        return lib.mssr_kv4_attention(ctypes.byref(c), q, 0, 0, 64, out, 0, 0, 64, H, Tq, lengths, n, 0, longest, 1.0, 0,
-                                      scratch, nbytes, dtype, None)
+        d = L.Kv4AttentionDesc(ctypes.addressof(c), q, 0, 0, 64, out, 0, 0, 64, Tq, lengths, n, longest, scratch, nbytes, H, 0,
+                               1.0, 0, dtype)
+        return lib.mssr_kv4_attention(ctypes.byref(d), None)
 
     for c in (cache(data=None), cache(dh=60), cache(dh=160), cache(B=0), cache(H=0), cache(capacity=0), cache(data=FAKE + 4)):
         assert call(c) == 1
@@ -103,6 +105,18 @@ def test_new_logits_overlap_the_old_ones_in_place_or_not_at_all():
         assert b"32-bit picks" in L.load().mssr_last_error(), kw
     for kw in (dict(ld=1 << 40), dict(ldo=1 << 40)):
         assert control(**kw) == 1, kw
+
+
+def test_packed_descriptors_lie_as_the_structures_do():
+    for desc in (L.Kv4Rows, L.Kv4AttentionDesc, L.TokenControlDesc):
+        fields = [1.25 * i if t is ctypes.c_float else 3 * i + 1 for i, (_, t) in enumerate(desc._fields_)]
+        packed = L.packer(desc)(*fields)
+        assert len(packed) == ctypes.sizeof(desc)
+        back = desc.from_buffer_copy(packed)
+        assert [getattr(back, name) for name, _ in desc._fields_] == fields
+    assert L.load().mssr_kv4_write(None, None) == 1 and L.load().mssr_kv4_read(None, None) == 1
+    assert L.load().mssr_kv4_attention(None, None) == 1
+    assert L.load().mssr_kv4_attention(bytes(ctypes.sizeof(L.Kv4AttentionDesc)), None) == 1
 
 
 def test_pack_allowed():
