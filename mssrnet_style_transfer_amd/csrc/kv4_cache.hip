@@ -106,8 +106,9 @@ struct Kv4WriteArgs {
     int64_t items;
 };
 
-// One group of one token: load, quantise, store straight to memory.  Few tokens a sentence: a token's bytes are
-// scattered over its block, nothing is gained by collecting them.
+// One group of one token: load, quantise, store straight to memory: a token's bytes are scattered over its block, which costs
+// little while there are few.  Bound by latency (512 sentences x 8 heads of 64 bf16 features, one token each: 4.3 us, 2.5 of
+// it an empty launch).
 template <typename T>
 __global__ __launch_bounds__(256) void kv4_write_tokens_kernel(Kv4WriteArgs a) {
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -149,7 +150,9 @@ __global__ __launch_bounds__(256) void kv4_write_tokens_kernel(Kv4WriteArgs a) {
 
 // One cache block of one (sentence, head): its image is put together in LDS and leaves in 16-byte stores where the call
 // covers the whole block, in the dwords and bytes of the covered tokens where it does not.  A thread has 8 features of four
-// consecutive tokens, so that the V codes, a byte a token, are dwords before they reach LDS.
+// consecutive tokens, so that the V codes, a byte a token, are dwords before they reach LDS.  Bound by memory and, closely, by
+// vector instructions: 64 heads x 8191 tokens of 128 bf16 features (268 MB in, 84 out) 92 us, 3.8 TB/s.  (Keys and values
+// requested together take 82 us instead of 66 for 8192 heads x 128 tokens: fewer waves fit.)
 template <typename T, int NG>
 __global__ __launch_bounds__(64 * NG) void kv4_write_blocks_kernel(Kv4WriteArgs a, uint32_t span) {
     constexpr int THREADS = 64 * NG;
@@ -258,6 +261,7 @@ __device__ __forceinline__ void kv4_decode(P img, int ng, int tok, int g, int qu
     }
 }
 
+// The same items the other way, 4.2 us for 4096 heads x 1 token.
 template <typename T>
 __global__ __launch_bounds__(256) void kv4_read_tokens_kernel(Kv4ReadArgs a) {
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -283,7 +287,8 @@ __global__ __launch_bounds__(256) void kv4_read_tokens_kernel(Kv4ReadArgs a) {
     Ld8<T>::store((T*)a.v + b * a.v_bs + h * a.v_hs + t * a.v_ts + ch, v);
 }
 
-// 64 output tokens of one (sentence, head); they lie in at most two cache blocks, whose images pass through LDS
+// 64 output tokens of one (sentence, head); they lie in at most two cache blocks, whose images pass through LDS.  Bound by
+// memory: 64 heads x 8191 tokens of 128 bf16 features 66 us, 5.3 TB/s.
 template <typename T, int NG>
 __global__ __launch_bounds__(256) void kv4_read_blocks_kernel(Kv4ReadArgs a, uint32_t span) {
     __shared__ __align__(16) uint8_t img[2 * NG * 2560];
@@ -356,8 +361,19 @@ extern "C" int64_t mssr_kv4_bytes(int64_t B, int H, int64_t capacity, int dh) {
     return B * H * per;
 }
 
-// tokens a sentence from which a call collects whole blocks in LDS
-static constexpr int64_t KV4_BLOCK_MIN_T = 16;
+// Whether a call goes token by token (else by blocks, through LDS).  Graph replays, us, tokens against blocks:
+//   writing: below 64 tokens a sentence no block is whole (8192 heads of 64 features: 2 tokens 6.1 against 56, 32 tokens 34
+//     against 58, 64 tokens 61 against 54, 128 tokens 127 against 66), and a block's work takes 5 us however few there are
+//     (64 heads x 192 tokens 4.6 against 6.1, 8 heads x 4000 tokens 7.3 against 7.6, but 256 heads of 128 features x 128
+//     tokens 11 against 8.2)
+//   reading: the other way round from 16 tokens on (8192 heads: 8 tokens 9.9 against 13, 16 tokens 15.7 against 14.0; 64
+//     heads x 16 tokens 2.8 against 2.5)
+// and what 32-bit item numbers hold.
+static bool kv4_by_tokens(int64_t bh, int64_t T, int ng, bool write) {
+    if (bh > (int64_t)1 << 27 || T >= (int64_t)1 << 26) return false;
+    const bool few = write ? T < KV4_TOK || bh * T * ng <= 1 << 16 : T < 16;
+    return few && bh * T * ng * 4 < (int64_t)1 << 31;
+}
 
 extern "C" int mssr_kv4_write(const mssr_kv4_rows* r, void* stream) {
     if (int rc = kv4_check_rows(r, "kv4_write")) return rc;
@@ -370,7 +386,7 @@ extern "C" int mssr_kv4_write(const mssr_kv4_rows* r, void* stream) {
     Kv4WriteArgs a{kv4_view(c), r->k, r->v, r->k_bs, r->k_hs, r->k_ts, r->v_bs, r->v_hs, r->v_ts, T,
                   {r->start, r->index_bits & 1, r->start0}, {r->counts, (r->index_bits >> 1) & 1, 0}, 0};
     const int64_t bh = c->B * c->H;
-    if (T < KV4_BLOCK_MIN_T && bh <= (int64_t)1 << 27 && bh * T * ng * 4 < (int64_t)1 << 31) {
+    if (kv4_by_tokens(bh, T, ng, true)) {
         a.items = bh * T * ng * 4;
         const unsigned grid = (unsigned)((a.items + 255) / 256);
         if (dtype == MSSR_F32) kv4_write_tokens_kernel<float><<<grid, 256, 0, s>>>(a);
@@ -402,7 +418,7 @@ extern "C" int mssr_kv4_read(const mssr_kv4_rows* r, void* stream) {
     Kv4ReadArgs a{kv4_view(c), r->k, r->v, r->k_bs, r->k_hs, r->k_ts, r->v_bs, r->v_hs, r->v_ts, T,
                   {r->start, r->index_bits & 1, r->start0}, {r->counts, (r->index_bits >> 1) & 1, 0}, 0};
     const int64_t bh = c->B * c->H;
-    if (T < KV4_BLOCK_MIN_T && bh <= (int64_t)1 << 27 && bh * T * ng * 4 < (int64_t)1 << 31) {
+    if (kv4_by_tokens(bh, T, ng, false)) {
         a.items = bh * T * ng * 4;
         const unsigned grid = (unsigned)((a.items + 255) / 256);
         if (dtype == MSSR_F32) kv4_read_tokens_kernel<float><<<grid, 256, 0, s>>>(a);

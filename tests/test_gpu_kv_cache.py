@@ -451,3 +451,31 @@ def test_scales_that_grow_along_the_sentence(kv, dtype, B, H, Hkv, dh, Tq, cap):
     n = [cap - 3 * b for b in range(B)]
     want, bound = attend(q, values(k), values(v), n, 1.0 / math.sqrt(dh), True)
     close(kv.attention(q, c, torch.tensor(n, device="cuda"), causal=True), want, bound, "growing scales")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dh", [24, 64, 88, 128])
+@pytest.mark.parametrize("T", [64, 70, 127, 200])
+def test_many_heads_at_once_write_the_same_bytes(kv, dtype, dh, T):
+    # 1120 heads go through whole blocks; the same tokens 40 at a time do not: every byte of the cache must agree
+    B, H, cap = 140, 8, 210
+    k, v = heads(B, H, T, dh, dtype, 71, 2.0), heads(B, H, T, dh, dtype, 72)
+    k[3, 1, 5, 0], k[4, 2, T - 1, dh - 1], v[5, 3, 9, 3], v[6, 0, 0, 1] = float("nan"), float("inf"), 1e30, -float("inf")
+    g = torch.Generator().manual_seed(T)
+    start = torch.randint(-5, cap - T // 2, (B,), generator=g)
+    start[:4] = torch.tensor([0, 64, -200, cap])
+    counts = torch.randint(0, T + 2, (B,), generator=g)
+    for st, n in ((0, None), (min(5, cap - T), None), (start.cuda(), None), (start.cuda(), counts.cuda())):
+        c, d = kv.KVCache4(B, H, dh, cap), kv.KVCache4(B, H, dh, cap)
+        for x in (c, d):
+            x.data.fill_(0xA5)
+        c.write(k, v, st, n)
+        for lo in range(0, T, 40):
+            hi = min(lo + 40, T)
+            d.write(k[:, :, lo:hi], v[:, :, lo:hi], st + lo, None if n is None else n - lo)
+        assert torch.equal(c.data, d.data)
+    got = c.read(start.cuda(), T, counts.cuda(), dtype=torch.float32)
+    for out, x in zip(got, (k, v)):
+        b = 10
+        lo, hi = max(0, -int(start[b])), min(T, int(counts[b]), cap - int(start[b]))
+        assert torch.equal(out[b, :, lo:hi], values(x[b, :, lo:hi]).float())
