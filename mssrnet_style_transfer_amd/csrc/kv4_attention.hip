@@ -61,7 +61,7 @@ constexpr float KV4_LAZY = 8.f;          // log2 of how far a probability may pa
 constexpr float KV4_UP = 7.f;            // log2 of what probabilities are held times
 constexpr float KV4_NONE = -3e38f;       // the reference of a row that has seen no token: 2^(-inf - KV4_NONE) is 0
 constexpr float KV4_MID = 7.5f;          // what fp32 calls take from codes and add, times the scale, to zeros
-constexpr int KV4_MAX_SPLITS = 512;
+constexpr int KV4_MAX_SPLITS = 256;
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -790,29 +790,31 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a) {
 struct Kv4Shape { int rows, W, splits; int64_t units; };
 
 // How a call is cut: `longest` bounds the lengths (the capacity where the caller knows no better), nb is that in blocks of
-// 64 tokens, units the (sentence, key/value head, query rows) triples.  Measured on graph replays, us:
-//   a wave each (W = 1) where units fill the chip: 4096 units of 140 tokens 12.5 against 18.7 with four waves; 2048 units
-//     of 1200 tokens 39.8 against 41.2, of more it evens out
-//   eight waves where units are few: 8 units of 1200 tokens 5.5 against 6.7 with four; 256 units of 5000 tokens 20 against
-//     25; but 512 units of 300 tokens 6.1 against 5.7, and many-row kernels on 512 units 10.9 against 8.0.  4 rows: 256
-//     units of 2500 tokens 15.1 against 18.6, but 64 of 300 tokens 6.4 against 5.9
-//   splits, whose joining costs a second launch (3 us), where a unit's waves would go round more than four times and the
-//     chip has room: 8 units of 5000 tokens 7.2 against 11.3; with 256 units of 10000 tokens 42 against 38 unsplit.  128
-//     units of 0 .. 32768 tokens: 8 splits 36, 2 splits 47.  4 rows, 64 units, as many splits as give 256 blocks: 8190
-//     tokens 17 against 27 (64 features), 32 against 61 (128, fp32); 1000 tokens 9.6 against 8.5 and 15.2 against 15.9
+// 64 tokens, units the (sentence, key/value head, query rows) triples.  Measured on graph replays, us, "a x b" for a units of b
+// tokens, 64 bf16 features unless others are named:
+//   a wave each (W = 1) where units fill the chip: 2048 x 140 7.6 against 11.0 with four waves, 4096 x 1200 with 16 rows 83
+//     against 97, with 4 rows (96 fp32 features) 131 against 160; with one row 2048 x 1200 31 against 29
+//   eight waves where units are few: 64 x 1200 6.1 against 7.4, 512 x 1200 11.8 against 12.5; but 512 x 300 6.1 against 5.7,
+//     512 x 2500 of 128 fp32 features 44 against 42, many-row kernels on 512 units 10.9 against 8.0.  4 rows: 256 x 2500 15.1
+//     against 18.6, but 64 x 300 6.4 against 5.9
+//   splits, whose joining costs a second launch (3 us), where a unit's waves would go round often and the chip has room: as
+//     many as give every CU a block, or two where two fit and there are several sentences (their lengths differ), and twice as
+//     many again for very long ones.  64 x 10000 15.3 against 25.4 unsplit (with 9 splits, blocks that do not fill the last
+//     round, 19.3), 128 fp32 features 24.7 against 46.1; 64 x 2500 9.0 against 8.2; 128 x 0 .. 32768 36 with 8 splits, 38
+//     with 4.  4 rows: 64 x 8190 17 against 27, of 128 fp32 features 32 against 61; 64 x 1000 9.6 against 8.5
 static Kv4Shape kv4_shape(int64_t B, int Hkv, int NQ, int ng, int64_t longest) {
     Kv4Shape s;
     s.rows = NQ == 1 ? 1 : NQ <= 4 ? 4 : 16;
     s.units = B * Hkv * ((NQ + s.rows - 1) / s.rows);
     const int64_t nb = (longest + KV4_TOK - 1) / KV4_TOK;
-    const bool crowd = s.units >= 2048 && nb <= 16;
-    const bool eight = s.rows == 4 ? nb >= 16 && s.units <= 256 : nb > 4 && (s.units <= 256 || (s.rows == 1 && nb >= 24));
-    s.W = nb <= 1 || crowd ? 1 : eight ? 8 : 4;
+    const bool lone = nb <= 1 ? s.rows == 1 || s.units >= 512 : s.units >= 2048 && nb <= (s.rows == 1 ? 16 : 24);
+    const bool eight = s.rows == 4    ? nb >= 16 && s.units <= 256
+                       : s.units <= 256 ? nb > 4
+                                        : s.rows == 1 && ng <= 2 && nb >= 16 && s.units <= 512;
+    s.W = lone ? 1 : eight ? 8 : 4;
     int64_t want = 1;
-    if (s.rows == 1 && nb >= 36 && s.units <= 128) {
-        const int64_t room = 1024 / s.units, use = nb / (8 * (1 + s.units / 64));
-        want = room < use ? room : use;
-    }
+    if (s.rows == 1 && s.units <= 128 && nb * ng >= 80 + s.units / 2)
+        want = (s.units < 64 ? 256 : (ng <= 2 ? 512 : 256) << (nb >= 256 ? 1 : 0)) / s.units;
     if (s.rows == 4 && nb * ng >= 48 + s.units / 4) want = 256 / s.units;
     if (s.rows == 16 && nb >= 20) want = 256 / s.units;
     const int64_t most = (nb + s.W - 1) / s.W;
