@@ -257,6 +257,12 @@ __device__ __forceinline__ void kv4_finish(const Kv4AttnArgs& a, const Kv4Work& 
 //   scores   per group 4 products of 16 tokens; every quad of rows of the q operand holds the same rows, so lane
 //            (quad, n) finds token n of each product and keeps the one of its own 16 (one fp32 row: its parts are rows)
 //   p s      goes through LDS to become an operand: row 4 part + r, the parts add up at the end
+// Bound by memory where sentences are long or many: 16 sentences x 8 heads x 26000 tokens of 64 bf16 features (270 MB) 43 us
+// and 5 for the join, 58 us in a row of launches, 4.6 TB/s, the rate of a large copy; 512 x 8 heads x 65 .. 140 tokens 12.1 us,
+// 3 of them the launch (35 MB needed, 40 read: half blocks are the least).  By vector instructions and latency elsewhere: 8 x 8
+// heads with 4 fp32 rows each, 4000 .. 8190 tokens of 128 features (63 MB) 24 us and 4 for the join, 9 of which a sentence of
+// one block takes as well (some 1500 instructions before and after the loop; in it 420 vector and 56 matrix ones a block); one
+// sentence of 20 tokens 3.3 us.
 template <typename T, int NG, int R, int W>
 __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnArgs a) {
     constexpr bool F32 = sizeof(T) == 4;
@@ -473,10 +479,13 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
 //   scores   tokens x queries: lane (quad, n) holds tokens 16 t + 4 quad + 0..3 of query n
 //   p s      is an operand as it lies (slots 0-3 from tile 2 ks, 4-7 from 2 ks + 1, the order of the V codes)
 //   context  features x queries: lane (quad, n) holds features 16 c + 4 quad + 0..3 of query n
-// Bound by vector instructions (16 scores a lane and block): what can be a product is one.  The zeros' share of a score,
-// sum_g z_tg Q_g, is a product of 8 slots (z exact in fp16, Q in two parts), sum_t p_t z_tg and sum_t p_t are rows of one
-// more product of p.  Scales and zeros are one a token and reach the lanes through LDS; a group that is NaN has a NaN
-// scale, its zero is taken as 0 so that rows that do not see the token stay clean.
+// Bound by vector instructions (16 scores a lane and block, 360 instructions at 96 features): what can be a product is one.
+// The zeros' share of a score, sum_g z_tg Q_g, is a product of 8 slots (z exact in fp16, Q in two parts), sum_t p_t z_tg and
+// sum_t p_t are rows of one more product of p.  Scales and zeros are one a token and reach the lanes through LDS; a group
+// that is NaN has a NaN scale, its zero is taken as 0 so that rows that do not see the token stay clean.
+// 24 x 4 heads with 20 rows each, 700 .. 2050 tokens of 96 bf16 features (17 MB): 15.6 us, 8 of which a sentence of one block
+// takes as well (18.6 with a second copy of the step for blocks without masks and with divisions: code that is run through
+// once is slow to fetch).
 template <typename T, int NG, int W>
 __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnArgs a) {
     constexpr bool F32 = sizeof(T) == 4;
@@ -745,6 +754,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
 }
 
 // Joins the splits of a query row: the factors once for all, then every wave a quarter of the splits, two features a lane.
+// Bound by latency: 4 us of which 3 are a launch's (requesting the first splits before the factors are made changes nothing).
 template <typename T>
 __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a) {
     __shared__ float fac[KV4_MAX_SPLITS], red[4][KV4_MAX_DH], sums[4];

@@ -8,6 +8,9 @@
 // Bound by memory: the logits once, written once or not at all.  A block owns a chunk of a row: it walks the history
 // first and marks the chunk's words in LDS (count, seen, banned; 16 bits a word while counts fit, so that a chunk can be
 // 32768 words: every chunk of a row walks the whole history), then streams the logits, 8 words a thread.
+// Measured: 128 rows x 50001 fp32 words, history 300, new logits (52 MB) 15.4 us, 3.4 TB/s; 64 x 131071 bf16, history 2000 with
+// 4-grams (35 MB) 13.9 us; the pick of 512 x 9606 bf16 (10 MB) 8.7 us and of one row 5.5 us, where latency counts: a launch 2.5,
+// the logits 1.4, the history's walk (clear, walk, two barriers) 1.1 (1.8 with two blocks a CU).
 #include "common.hpp"
 #include "kv4.hpp"      // IdxTable
 
