@@ -479,3 +479,52 @@ def test_many_heads_at_once_write_the_same_bytes(kv, dtype, dh, T):
         b = 10
         lo, hi = max(0, -int(start[b])), min(T, int(counts[b]), cap - int(start[b]))
         assert torch.equal(out[b, :, lo:hi], values(x[b, :, lo:hi]).float())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,H,Hkv,dh,Tq,cap", [
+    (256, 8, 8, 64, 1, 140),        # a wave each: one row
+    (256, 32, 8, 32, 1, 200),       # four rows
+    (256, 8, 8, 40, 5, 150),        # sixteen
+    (128, 8, 4, 96, 1, 60),         # 512 heads of one block, two rows
+    (40, 8, 8, 64, 9, 60),          # 320 of sixteen rows
+    (8, 8, 8, 64, 1, 1700),         # eight waves, unsplit
+    (64, 8, 8, 64, 1, 1100),
+    (32, 8, 8, 128, 1, 400),
+    (6, 8, 8, 64, 1, 6000),         # split: one row,
+    (3, 16, 4, 128, 1, 2600),       # four,
+    (2, 8, 4, 64, 6, 2500),         # sixteen
+])
+def test_every_way_a_call_is_cut(kv, dtype, B, H, Hkv, dh, Tq, cap):
+    g = torch.Generator().manual_seed(B + cap)
+    n = torch.randint(0, cap + 1, (B,), generator=g)
+    n[0], n[-1] = cap, cap - 1
+    k, v, q = heads(B, Hkv, cap, dh, dtype, 41, 0.7), heads(B, Hkv, cap, dh, dtype, 42), heads(B, H, Tq, dh, dtype, 43)
+    c = kv.KVCache4(B, Hkv, dh, cap)
+    c.data.fill_(0xFF)                                  # past the lengths: NaN scales
+    c.write(k, v, 0, n.cuda())
+    got = kv.attention(q, c, n.cuda(), causal=True)
+    assert torch.isfinite(got).all()
+    for b in sorted({0, 1, B // 2, B - 1}):
+        at = slice(b, b + 1)
+        want, bound = attend(q[at], values(k[at]), values(v[at]), n[at].tolist(), 1.0 / math.sqrt(dh), True)
+        close(got[at], want, bound, "sentence %d of %d tokens" % (b, int(n[b])))
+
+
+def test_two_calls_at_once(kv):
+    # both are split, so both use scratch; each has its own
+    k, v = heads(2, 4, 9000, 64, torch.float32, 31), heads(2, 4, 9000, 64, torch.float32, 32)
+    c = kv.KVCache4(2, 4, 64, 9000)
+    c.write(k, v)
+    q = [heads(2, 4, 1, 64, torch.float32, 33 + i) for i in range(2)]
+    want = [kv.attention(x, c, 9000 - 100 * i) for i, x in enumerate(q)]
+    streams = [torch.cuda.Stream() for _ in q]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(kv.attention(q[i], c, 9000 - 100 * i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])

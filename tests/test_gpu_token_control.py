@@ -309,3 +309,21 @@ def test_a_batch_without_rows(tc):
     x = torch.zeros(0, 40, device="cuda")
     each = tc.TokenControl(allowed=torch.zeros(0, 2, dtype=torch.int32, device="cuda"))
     assert tc.control_logits(x, each).shape == (0, 40) and tc.pick_token(x, each).shape == (0,)
+
+
+def test_two_picks_at_once(tc):
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x = [torch.randn(3, 50000, device="cuda", generator=g) for _ in range(2)]           # several chunks a row: scratch
+    h = torch.randint(0, 50000, (3, 40), device="cuda", generator=g)
+    c = tc.TokenControl(repetition=1.3, ngram=1)
+    want = [tc.pick_token(t, c, h) for t in x]
+    streams = [torch.cuda.Stream() for _ in x]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(tc.pick_token(x[i], c, h))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(t, want[i]) for t in got[i])
