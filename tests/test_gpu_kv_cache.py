@@ -494,6 +494,8 @@ def test_many_heads_at_once_write_the_same_bytes(kv, dtype, dh, T):
     (6, 8, 8, 64, 1, 6000),         # split: one row,
     (3, 16, 4, 128, 1, 2600),       # four,
     (2, 8, 4, 64, 6, 2500),         # sixteen
+    (2, 8, 2, 128, 5, 700),         # the largest block: eight waves of sixteen rows and 128 features
+    (1, 8, 2, 128, 5, 2000),
 ])
 def test_every_way_a_call_is_cut(kv, dtype, B, H, Hkv, dh, Tq, cap):
     g = torch.Generator().manual_seed(B + cap)
@@ -505,7 +507,7 @@ def test_every_way_a_call_is_cut(kv, dtype, B, H, Hkv, dh, Tq, cap):
     c.write(k, v, 0, n.cuda())
     got = kv.attention(q, c, n.cuda(), causal=True)
     assert torch.isfinite(got).all()
-    for b in sorted({0, 1, B // 2, B - 1}):
+    for b in sorted({0, min(1, B - 1), B // 2, B - 1}):
         at = slice(b, b + 1)
         want, bound = attend(q[at], values(k[at]), values(v[at]), n[at].tolist(), 1.0 / math.sqrt(dh), True)
         close(got[at], want, bound, "sentence %d of %d tokens" % (b, int(n[b])))
@@ -528,3 +530,14 @@ def test_two_calls_at_once(kv):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+@pytest.mark.parametrize("longest", [1, 64, 700, 1 << 40])
+def test_longest_shapes_the_launch_and_nothing_else(kv, longest):
+    for H, Tq in ((2, 1), (8, 1), (4, 7)):
+        k, v, q = (heads(2, h, t, 64, torch.float32, s) for h, t, s in ((2, 3000, 51), (2, 3000, 52), (H, Tq, 53)))
+        c = kv.KVCache4(2, 2, 64, 3000)
+        c.write(k, v)
+        n = torch.tensor([3000, 1234], device="cuda")
+        want, bound = attend(q, values(k), values(v), n, 1 / 8, False)
+        close(kv.attention(q, c, n, longest=longest), want, bound, "longest %d" % longest)
