@@ -8,18 +8,22 @@
 // c * 2^-24 (subnormals, which the matrix cores keep), so `x & 0x000f000f` IS an operand pair and `x & 0x00f000f0` one
 // that is 16 times as large.  8 codes take 5 vector instructions.  (The matrix cores align a subnormal's bits as if its
 // leading one stood in place: with codes in the lowest four of ten bits, products lose what is below 2^-21 of the largest.
-// bf16 calls do not see it; fp32 ones take all codes 16 times as large, 2^-26, for two shifts more.)
+// bf16 scores do not see it; where it counts all codes are 16 times as large, 2^-26, for two shifts more.)
 //
-// What meets the codes is fp16 too (11 bits), as parts whose products add up in fp32: one part for bf16 calls (exact for
-// q; 2^-11 of p s, averaged over tokens, where the result keeps 2^-8), two for fp32 ones (2^-22).  Powers of two keep
+// What meets the codes is fp16 too (11 bits), as parts whose products add up in fp32: q one part in bf16 calls (exact), two in
+// fp32 ones (2^-22); p s two (2^-22) in either (one in bf16 calls of more than 4 rows).  One part would keep 2^-12 of the codes'
+// share, which the zeros' share nearly cancels: of a single token's stored values, which come back then, one in five was not the
+// nearest bf16 number, and of values about zero one in three.  Powers of two keep
 // them in fp16's range: a query row is scaled to a largest element in [2^13, 2^14); p s is taken relative to the largest
 // V scale met so far (rounded up to a power of two; when it grows, the sums shrink), with p up to 2^8 (below) and 7 bits
 // on top, so that what is 2^-21 of the largest still has all its bits and the rest is off by at most 2^-32 of it.
 //
 // Where values are spread about zero, codes' and zeros' shares of the context nearly cancel, the more so the more tokens
-// there are, and a product's sums are cut, not rounded, where they meet an accumulator that has outgrown them.  fp32 calls
-// therefore take 7.5 from every code (one more product against a constant) and add 7.5 s to every zero, and start each
-// block of 64 tokens from zero, added up by rounding additions: 1000 .. 16000 tokens of mean zero come out within 1e-6.
+// there are, and a product's sums are cut, not rounded, where they meet an accumulator that has outgrown them.  7.5 is
+// therefore taken from every code (one more product against a constant) and 7.5 s added to every zero, and each block of 64
+// tokens starts from zero, added up by rounding additions (not so in bf16 calls of more than 4 rows): fp32 results of 3 .. 16000
+// tokens of mean zero come out within 1.1e-6 in norm, of bf16 ones 1 in 1000 is not the nearest (1 in 40 for a single token,
+// whose values often lie halfway between two).
 //
 // A wave takes 64 tokens at a time; the running maximum moves only when a score passes it by more than 8 (then every
 // sum is rescaled), so that a block of tokens costs one comparison and no cross-lane reduction.  The W waves of a block
@@ -60,7 +64,8 @@ struct Kv4AttnArgs {
 constexpr float KV4_LAZY = 8.f;          // log2 of how far a probability may pass 1 before a rescale
 constexpr float KV4_UP = 7.f;            // log2 of what probabilities are held times
 constexpr float KV4_NONE = -3e38f;       // the reference of a row that has seen no token: 2^(-inf - KV4_NONE) is 0
-constexpr float KV4_MID = 7.5f;          // what fp32 calls take from codes and add, times the scale, to zeros
+constexpr float KV4_MID = 7.5f;          // what is taken from codes and added, times the scale, to zeros
+constexpr int KV4_PS_PARTS = 2;          // fp16 parts of p s
 constexpr int KV4_MAX_SPLITS = 256;
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -270,7 +275,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
     constexpr bool QROWS = F32 && R == 1;        // the parts of q in rows of one product instead of products of their own
     constexpr int PLD = 72;                      // fp16 elements of an LDS row of 64 tokens: 16-byte reads of 16 rows spread
     constexpr int DP = NG * 32;
-    __shared__ __align__(16) uint16_t ps_[kv4_waves(W)][NG][PARTS * R][PLD];
+    __shared__ __align__(16) uint16_t ps_[kv4_waves(W)][NG][KV4_PS_PARTS * R][PLD];
     __shared__ float om_[kv4_waves(W) / W][W][R][DP + 4];
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = W == 1 ? 0 : wave;
@@ -416,11 +421,10 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
             for (int g = 0; g < NG; ++g) {
                 const uint32_t mvr = mv[g] & mask[r];
                 float y = p * kv4_scale(mvr);
-                if (F32) kv4_pin(y);
-                const float z = F32 ? fmaf(KV4_MID, kv4_scale(mvr), kv4_zero(mvr)) : kv4_zero(mvr);
-                zs[r][g] = fmaf(p, z, zs[r][g]);
+                kv4_pin(y);
+                zs[r][g] = fmaf(p, fmaf(KV4_MID, kv4_scale(mvr), kv4_zero(mvr)), zs[r][g]);
 #pragma unroll
-                for (int part = 0; part < PARTS; ++part) {
+                for (int part = 0; part < KV4_PS_PARTS; ++part) {
                     const f16 h = (f16)y;
                     y -= (float)h;
                     ps[g][part * R + r][col] = __builtin_bit_cast(uint16_t, h);
@@ -428,24 +432,24 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
             }
         }
         __builtin_amdgcn_wave_barrier();
-        // rows 4 part + r; the rows of absent parts and queries repeat others and are not used
-        const int row = R == 1 ? (PARTS == 2 ? (n >> 2) & 1 : 0) : (PARTS == 2 ? n & 7 : n & 3);
+        // rows 4 part + r; the rows past them, and of absent queries, repeat others and are not used
+        const int row = R == 1 ? (n >> 2) & 1 : n & 7;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            f32x4 c0 = F32 ? zero4 : acc[2 * g], c1 = F32 ? zero4 : acc[2 * g + 1], mid = zero4;
+            f32x4 c0 = zero4, c1 = zero4, mid = zero4;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
                 const int d = (ks * NG + g) * 2;
                 f16x8 lo, hi;
-                kv4_v_operands<F32>(cur.v[d >> 2][d & 3], cur.v[d >> 2][(d & 3) + 1], lo, hi);
+                kv4_v_operands<true>(cur.v[d >> 2][d & 3], cur.v[d >> 2][(d & 3) + 1], lo, hi);
                 const u32x4 raw = *reinterpret_cast<const u32x4*>(&ps[g][row][ks * 32 + quad * 8]);
                 const f16x8 pop = __builtin_bit_cast(f16x8, raw);
                 c0 = kv4_mfma(pop, lo, c0);
                 c1 = kv4_mfma(pop, hi, c1);
-                if (F32) mid = kv4_mfma(pop, kv4_mid(), mid);
+                mid = kv4_mfma(pop, kv4_mid(), mid);
             }
-            acc[2 * g] = F32 ? acc[2 * g] + (c0 + mid) : c0;
-            acc[2 * g + 1] = F32 ? acc[2 * g + 1] + (c1 + mid) : c1;
+            acc[2 * g] += c0 + mid;
+            acc[2 * g + 1] += c1 + mid;
         }
         __builtin_amdgcn_wave_barrier();
         if (more) cur.load_v(ahead, lane, wk.len - at - W * KV4_TOK);
@@ -460,8 +464,8 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
 #pragma unroll
         for (int c = 0; c < 2 * NG; ++c) {
             float u = acc[c][r];
-            if (PARTS == 2) u += __shfl_xor(u, 16);             // quads 0 and 1
-            u = fmaf(u, F32 || (c & 1) ? 0x1p20f : 0x1p24f, zt[c >> 1]);
+            u += __shfl_xor(u, 16);                             // quads 0 and 1
+            u = fmaf(u, 0x1p20f, zt[c >> 1]);
             if (quad == 0) om[w][r][c * 16 + n] = u;
         }
         if (lane == 0) {

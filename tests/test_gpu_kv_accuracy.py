@@ -1,0 +1,89 @@
+"""How near attention over the 4-bit cache comes to the formula in 64 bits over the values that the cache stands for, judged
+by what typical roundings add up to (tests/test_gpu_kv_cache.py bounds the worst case, which is far wider)."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_kv_cache import heads, values
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def kv():
+    from mssrnet_style_transfer_amd import kv_cache
+    with torch.no_grad():
+        yield kv_cache
+
+
+def exact(q, k, v, scale, visible=None):
+    """softmax(scale q k^T) v in 64 bits; k, v [B, Hkv, n, dh] in 64 bits already; visible: Bool [B, Tq, n], rows that see
+    something."""
+    B, H, T, dh = q.shape
+    G = H // k.shape[1]
+    s = torch.matmul(q.double(), k.repeat_interleave(G, 1).transpose(2, 3).contiguous()) * scale
+    if visible is not None:
+        s = s.masked_fill(~visible.unsqueeze(1), float("-inf"))
+    return torch.matmul(torch.softmax(s, -1), v.repeat_interleave(G, 1))
+
+
+def judge(got, want, share):
+    """``share``: how large the error before the result's rounding may be, as a part of the result's norm.
+
+    fp32: that, and the rounding itself (2^-24).  bf16: an error e moves a number over the border between two roundings with
+    probability |e| / ulp, ulp >= 2^-8 |x|.  With E|e| = 0.8 rms(e) and E min(ulp, .) / |x| about 5 / rms(x) for normally
+    distributed x, a share of 2^8 * 5 * 0.8 * share ~ 1024 share of the numbers; twice that is allowed."""
+    assert torch.isfinite(got).all()
+    if got.dtype == torch.float32:
+        err = float((got.double() - want).norm() / want.norm())
+        assert err <= share + 2.0 ** -24, "%.3g of the result, %.3g allowed" % (err, share)
+    else:
+        off = float((got != want.float().bfloat16()).double().mean())       # (rounded twice: moves one in 2^16)
+        assert off <= 2048 * share + 2 / got.numel(), "%.3g of the numbers are not the nearest, %.3g allowed" % (off, 2048 * share)
+
+
+ROWS = [(2, 2, 1), (8, 2, 1)]           # query heads, key/value heads, new tokens: one query row a head, four
+
+
+def check_one_token(kv, dtype, dh, H, Hkv, Tq):
+    B = 64
+    k, v, q = heads(B, Hkv, 1, dh, dtype, 1), heads(B, Hkv, 1, dh, dtype, 2), heads(B, H, Tq, dh, dtype, 3)
+    c = kv.KVCache4(B, Hkv, dh, 1)
+    c.write(k, v)
+    want = values(v).repeat_interleave(H // Hkv, 1).expand(B, H, Tq, dh)
+    # p cancels in the quotient; codes and zeros meet as |z| + 15 s <= 3 max |v| of the group, each held to 2^-22 and summed in
+    # half a dozen roundings: 2^-19 of the group's largest value, then the result's own rounding
+    top = torch.cat([g.abs().amax(-1, keepdim=True).expand_as(g) for g in want.split(32, -1)], -1)
+    half = torch.finfo(dtype).eps / 2
+    err = (kv.attention(q, c, 1).double() - want).abs()
+    assert (err <= 2.0 ** -19 * top + half * want.abs()).all(), float((err / (2.0 ** -19 * top + half * want.abs())).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dh", [8, 40, 64, 96, 128])
+@pytest.mark.parametrize("H,Hkv,Tq", ROWS)
+def test_a_sentence_of_one_token_is_that_token(kv, dtype, dh, H, Hkv, Tq):
+    check_one_token(kv, dtype, dh, H, Hkv, Tq)
+
+
+def check_mean_zero(kv, dtype, n, H, Hkv, Tq, same):
+    """Values about zero: the codes' and the zeros' share of the context cancel to 1 / sqrt(n) of either, and what is
+    cut off each time 64 tokens are added up does not average out: 2.4e-7 sqrt(n) (7.5 s = 2 deviations, 2^-24 each), over 1e-5 of
+    the parts' 2^-21 times 4 deviations and the scores' roundings."""
+    B, dh = 2 if n > 1000 else 16, 64
+    k, v, q = heads(B, Hkv, n, dh, dtype, 11), heads(B, Hkv, n, dh, dtype, 12), heads(B, H, Tq, dh, dtype, 13)
+    if same:
+        k = k[:, :, :1].expand(B, Hkv, n, dh)           # every token has the same score
+    c = kv.KVCache4(B, Hkv, dh, n)
+    c.write(k, v)
+    want = exact(q, values(k), values(v), 1 / math.sqrt(dh))
+    judge(kv.attention(q, c, n), want, 1e-5 + 2.4e-7 * math.sqrt(n))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("same", [False, True])
+@pytest.mark.parametrize("n", [3, 100, 2000, 16000])
+@pytest.mark.parametrize("H,Hkv,Tq", ROWS)
+def test_values_about_zero(kv, dtype, n, H, Hkv, Tq, same):
+    check_mean_zero(kv, dtype, n, H, Hkv, Tq, same)
