@@ -11,7 +11,7 @@
 // bf16 scores do not see it; where it counts all codes are 16 times as large, 2^-26, for two shifts more.)
 //
 // What meets the codes is fp16 too (11 bits), as parts whose products add up in fp32: q one part in bf16 calls (exact), two in
-// fp32 ones (2^-22); p s two (2^-22) in either (one in bf16 calls of more than 4 rows).  One part would keep 2^-12 of the codes'
+// fp32 ones (2^-22); p s two (2^-22) in either.  One part would keep 2^-12 of the codes'
 // share, which the zeros' share nearly cancels: of a single token's stored values, which come back then, one in five was not the
 // nearest bf16 number, and of values about zero one in three.  Powers of two keep
 // them in fp16's range: a query row is scaled to a largest element in [2^13, 2^14); p s is taken relative to the largest
@@ -21,9 +21,8 @@
 // Where values are spread about zero, codes' and zeros' shares of the context nearly cancel, the more so the more tokens
 // there are, and a product's sums are cut, not rounded, where they meet an accumulator that has outgrown them.  7.5 is
 // therefore taken from every code (one more product against a constant) and 7.5 s added to every zero, and each block of 64
-// tokens starts from zero, added up by rounding additions (not so in bf16 calls of more than 4 rows): fp32 results of 3 .. 16000
-// tokens of mean zero come out within 1.1e-6 in norm, of bf16 ones 1 in 1000 is not the nearest (1 in 40 for a single token,
-// whose values often lie halfway between two).
+// tokens starts from zero, added up by rounding additions: fp32 results of 1 .. 16000 tokens of mean zero come out within 1.1e-6
+// in norm, and of bf16 ones 1 or 2 in 1000 are not the nearest number.
 //
 // A wave takes 64 tokens at a time; the running maximum moves only when a score passes it by more than 8 (then every
 // sum is rescaled), so that a block of tokens costs one comparison and no cross-lane reduction.  The W waves of a block
@@ -103,6 +102,34 @@ __device__ __forceinline__ f32x4 kv4_mfma(f16x8 a, f16x8 b, f32x4 c) {
 // Makes a product the fp32 number it is: left alone, the compiler rounds it to fp16 here in one step and there in two, and the
 // second part is now and then the rest of another first part.
 __device__ __forceinline__ void kv4_pin(float& y) { asm volatile("" : "+v"(y)); }
+
+// Four p s -> half h of their two parts' operands (tokens in the order 0 2 1 3).  bf16 calls cut both parts, two numbers an
+// instruction: 2^-20, the same way for all, where the result keeps 2^-8.
+template <bool ROUND>
+__device__ __forceinline__ void kv4_split(float (&y)[4], f16x8& first, f16x8& second, int h) {
+    typedef __fp16 h2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        float &a = y[j], &b = y[j + 2];
+        if (ROUND) {
+            kv4_pin(a);
+            kv4_pin(b);
+            const f16 x = (f16)a, z = (f16)b;
+            first[4 * h + 2 * j] = x;
+            first[4 * h + 2 * j + 1] = z;
+            second[4 * h + 2 * j] = (f16)(a - (float)x);
+            second[4 * h + 2 * j + 1] = (f16)(b - (float)z);
+        } else {
+            const h2 x = __builtin_amdgcn_cvt_pkrtz(a, b);
+            const h2 z = __builtin_amdgcn_cvt_pkrtz(a - (float)x[0], b - (float)x[1]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                first[4 * h + 2 * j + e] = (f16)x[e];
+                second[4 * h + 2 * j + e] = (f16)z[e];
+            }
+        }
+    }
+}
 
 // 2^x of a whole number: references of exponents are whole, so that moving one rounds no sum (codes' and zeros' shares of
 // the context cancel: rounded apart, an fp32 result of 1000 tokens was off by 1e-5)
@@ -483,12 +510,14 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
 //   scores   tokens x queries: lane (quad, n) holds tokens 16 t + 4 quad + 0..3 of query n
 //   p s      is an operand as it lies (slots 0-3 from tile 2 ks, 4-7 from 2 ks + 1, the order of the V codes)
 //   context  features x queries: lane (quad, n) holds features 16 c + 4 quad + 0..3 of query n
-// Bound by vector instructions (16 scores a lane and block, 360 instructions at 96 features): what can be a product is one.
-// The zeros' share of a score, sum_g z_tg Q_g, is a product of 8 slots (z exact in fp16, Q in two parts), sum_t p_t z_tg and
-// sum_t p_t are rows of one more product of p.  Scales and zeros are one a token and reach the lanes through LDS; a group
-// that is NaN has a NaN scale, its zero is taken as 0 so that rows that do not see the token stay clean.
-// 24 x 4 heads with 20 rows each, 700 .. 2050 tokens of 96 bf16 features (17 MB): 15.6 us, 8 of which a sentence of one block
-// takes as well (18.6 with a second copy of the step for blocks without masks and with divisions: code that is run through
+// Bound by vector instructions (16 scores a lane and block): what can be a product is one, where that rounds nothing that
+// cancels.  The zeros' share of a score, sum_g z_tg Q_g, is a product of 8 slots (z exact in fp16, Q in two parts).  The sums of p
+// and of p (z + 7.5 s) are fp32 ones of the same p that p s is made of: with p rounded to fp16 in one of them, tokens of equal
+// score shared its error, and values about zero came out 2 % (2000 tokens) to 5 % (16000) off.  Scales and zeros are one a
+// token and reach the lanes through LDS; a group that is NaN has a NaN scale, its zero is taken as 0 so that rows that do not see
+// the token stay clean.
+// 24 x 4 heads with 20 rows each, 700 .. 2050 tokens of 96 bf16 features (17 MB): 18.9 us; 15.6 with one part of p s, 8 of
+// which a sentence of one block took as well (18.6 then with a second copy of the step for blocks without masks and with divisions: code that is run through
 // once is slow to fetch).
 template <typename T, int NG, int W>
 __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnArgs a) {
@@ -498,9 +527,8 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
     struct Token {
         float vs[NG][KV4_TOK];              // V scales * 2^-exponent
         uint16_t ks[NG][KV4_TOK];           // K scales
-        uint16_t vz[NG][KV4_TOK];           // V zeros in the operand's token order
         uint2 kz[KV4_TOK];                  // K zeros, groups 0..3
-        float vm[F32 ? NG : 1][KV4_TOK];    // fp32 calls: V zeros and KV4_MID V scales
+        float vm[NG][KV4_TOK];              // V zeros and KV4_MID V scales
     };
     __shared__ __align__(16) Token tk[kv4_waves(W)];
     __shared__ float om_[kv4_waves(W) / W][W][16][DP + 4];
@@ -546,13 +574,12 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
     bool fresh = true;
     float vtop = 0.f;                            // the largest V scale met; scales are taken times 2^-vexp, which bounds it
     int vexp = 0;
-    f32x4 acc[2 * NG], accz = {0.f, 0.f, 0.f, 0.f};         // accz: quad 0: sum p z_g, quad 1: sum p
-    float zs[F32 ? NG : 1];
+    f32x4 acc[2 * NG];
+    float zs[NG], l = 0.f;                       // of this lane's tokens
 #pragma unroll
-    for (int g = 0; g < (F32 ? NG : 1); ++g) zs[g] = 0.f;
+    for (int g = 0; g < NG; ++g) zs[g] = 0.f;
 #pragma unroll
     for (int c = 0; c < 2 * NG; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int col = (lane & 32) | ((lane & 12) << 1) | ((lane & 16) >> 2) | ((lane & 1) << 1) | ((lane >> 1) & 1);
     const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
     Token& my = tk[wave];
 
@@ -608,9 +635,9 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
             const float f = fresh ? 1.f : kv4_pow2(-up);
             fresh = fresh && !(top > -INFINITY);
             m += up;
-            accz *= f;
+            l *= f;
 #pragma unroll
-            for (int g = 0; g < (F32 ? NG : 1); ++g) zs[g] *= f;
+            for (int g = 0; g < NG; ++g) zs[g] *= f;
 #pragma unroll
             for (int c = 0; c < 2 * NG; ++c) acc[c] *= f * shrink;
 #pragma unroll
@@ -627,8 +654,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
         for (int g = 0; g < NG; ++g) {
             const float vz = kv4_zero(mv[g]);
             my.vs[g][lane] = kv4_scale(mv[g]) * vmul;
-            my.vz[g][col] = vz == vz ? (uint16_t)(mv[g] >> 16) : (uint16_t)0;
-            if (F32) my.vm[F32 ? g : 0][lane] = vz == vz ? fmaf(KV4_MID, kv4_scale(mv[g]), vz) : 0.f;
+            my.vm[g][lane] = vz == vz ? fmaf(KV4_MID, kv4_scale(mv[g]), vz) : 0.f;
         }
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -637,73 +663,45 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
             for (int r = 0; r < 4; ++r) {
                 s[t][r] = __builtin_amdgcn_exp2f(s[t][r]);
             }
-        // operand order of four tokens: 0 2 1 3
-        const uint32_t one2 = n == 4 ? 0x3c003c00u : 0u;
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            f16x8 pop[PARTS];
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float y = s[2 * ks + h][(j >> 1) | ((j & 1) << 1)];
-#pragma unroll
-                    for (int part = 0; part < PARTS; ++part) {
-                        const f16 b = (f16)y;
-                        y -= (float)b;
-                        pop[part][4 * h + j] = b;
-                    }
-                }
-            u32x4 zop = {one2, one2, one2, one2};
-            if (!F32 && n < NG) zop = *reinterpret_cast<const u32x4*>(&my.vz[n < NG ? n : 0][32 * ks + 8 * quad]);
-#pragma unroll
-            for (int part = 0; part < PARTS; ++part) accz = kv4_mfma(__builtin_bit_cast(f16x8, zop), pop[part], accz);
-        }
+        for (int t = 0; t < 4; ++t) l += (s[t][0] + s[t][1]) + (s[t][2] + s[t][3]);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            f32x4 c[PARTS][2], mid = zero4;      // one accumulator a part: the smaller part's sums would be cut in the larger's
+            // fp32 calls: one accumulator a part, the smaller part's sums would be cut in the larger's (4.7e-6 of 16000 tokens'
+            // mean-zero result against 8e-7; bf16 ones have 20 to 40 registers less to spill)
+            f32x4 c[PARTS][2], mid = zero4;
 #pragma unroll
-            for (int part = 0; part < PARTS; ++part) {
-                c[part][0] = F32 ? zero4 : acc[2 * g];
-                c[part][1] = F32 ? zero4 : acc[2 * g + 1];
-            }
+            for (int part = 0; part < PARTS; ++part) c[part][0] = c[part][1] = zero4;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-                f16x8 pop[PARTS];
+                f16x8 pop[KV4_PS_PARTS];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int t = 2 * ks + h;
                     const f32x4 v4 = *reinterpret_cast<const f32x4*>(&my.vs[g][16 * t + 4 * quad]);
-                    f32x4 z4 = zero4;
-                    if (F32) z4 = *reinterpret_cast<const f32x4*>(&my.vm[F32 ? g : 0][16 * t + 4 * quad]);
+                    const f32x4 z4 = *reinterpret_cast<const f32x4*>(&my.vm[g][16 * t + 4 * quad]);
+                    float y[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int r = (j >> 1) | ((j & 1) << 1);
-                        if (F32) zs[F32 ? g : 0] = fmaf(s[t][r], z4[r], zs[F32 ? g : 0]);
-                        float y = s[t][r] * v4[r];
-                        if (__builtin_expect(hidden, 0)) y = 16 * t + 4 * quad + r < see ? y : 0.f;
-                        if (F32) kv4_pin(y);
-#pragma unroll
-                        for (int part = 0; part < PARTS; ++part) {
-                            const f16 b = (f16)y;
-                            y -= (float)b;
-                            pop[part][4 * h + j] = b;
-                        }
+                    for (int r = 0; r < 4; ++r) {
+                        zs[g] = fmaf(s[t][r], z4[r], zs[g]);
+                        y[r] = s[t][r] * v4[r];
+                        if (__builtin_expect(hidden, 0)) y[r] = 16 * t + 4 * quad + r < see ? y[r] : 0.f;
                     }
+                    kv4_split<F32>(y, pop[0], pop[1], h);
                 }
                 const int d = (ks * NG + g) * 2;
                 f16x8 lo, hi;
-                kv4_v_operands<F32>(cur.v[d >> 2][d & 3], cur.v[d >> 2][(d & 3) + 1], lo, hi);
+                kv4_v_operands<true>(cur.v[d >> 2][d & 3], cur.v[d >> 2][(d & 3) + 1], lo, hi);
 #pragma unroll
-                for (int part = 0; part < PARTS; ++part) {
-                    c[part][0] = kv4_mfma(lo, pop[part], c[part][0]);
-                    c[part][1] = kv4_mfma(hi, pop[part], c[part][1]);
-                    if (F32) mid = kv4_mfma(kv4_mid(), pop[part], mid);
+                for (int part = 0; part < KV4_PS_PARTS; ++part) {
+                    c[part % PARTS][0] = kv4_mfma(lo, pop[part], c[part % PARTS][0]);
+                    c[part % PARTS][1] = kv4_mfma(hi, pop[part], c[part % PARTS][1]);
+                    mid = kv4_mfma(kv4_mid(), pop[part], mid);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) acc[2 * g + h] = F32 ? acc[2 * g + h] + (c[0][h] + mid + c[PARTS - 1][h]) : c[0][h];
+            for (int h = 0; h < 2; ++h) acc[2 * g + h] += PARTS == 2 ? c[0][h] + mid + c[PARTS - 1][h] : c[0][h] + mid;
         }
     };
 
@@ -734,23 +732,22 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
         if (more) cur.load_v(ahead, lane);
     }
 
-    const float unit = __builtin_amdgcn_ldexpf(1.f, 24 + vexp);
+    const float unit = __builtin_amdgcn_ldexpf(1.f, 20 + vexp);
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-        float z = F32 ? zs[F32 ? g : 0] : __shfl(accz[g], n);
-        if (F32) {
-            z += __shfl_xor(z, 16);
-            z += __shfl_xor(z, 32);
-        }
+        float z = zs[g];
+        z += __shfl_xor(z, 16);
+        z += __shfl_xor(z, 32);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                om[w][n][g * 32 + h * 16 + quad * 4 + r] = fmaf(acc[2 * g + h][r], F32 || h ? unit / 16.f : unit, z);
+            for (int r = 0; r < 4; ++r) om[w][n][g * 32 + h * 16 + quad * 4 + r] = fmaf(acc[2 * g + h][r], unit, z);
     }
     if (quad == 1) {
         om[w][n][DP] = fresh ? -INFINITY : m;
-        om[w][n][DP + 1] = accz[0];
+        om[w][n][DP + 1] = l;
     }
     if (W > 1) __syncthreads();
     else __builtin_amdgcn_wave_barrier();

@@ -39,7 +39,10 @@ def judge(got, want, share):
         err = float((got.double() - want).norm() / want.norm())
         assert err <= share + 2.0 ** -24, "%.3g of the result, %.3g allowed" % (err, share)
     else:
-        off = float((got != want.float().bfloat16()).double().mean())       # (rounded twice: moves one in 2^16)
+        # Stored values lie on a grid, so that means of a few of equal weight often lie halfway between two bf16 numbers, both
+        # of them nearest then: 9 % of single values, 4 % of means of three, 0.5 % of means of a hundred (counted in 64 bits).
+        least = (want.float().bfloat16().double() - want).abs()             # (rounded twice: moves one in 2^16)
+        off = float(((got.double() - want).abs() > least * (1 + 1e-9)).double().mean())
         assert off <= 2048 * share + 2 / got.numel(), "%.3g of the numbers are not the nearest, %.3g allowed" % (off, 2048 * share)
 
 
@@ -86,4 +89,22 @@ def check_mean_zero(kv, dtype, n, H, Hkv, Tq, same):
 @pytest.mark.parametrize("n", [3, 100, 2000, 16000])
 @pytest.mark.parametrize("H,Hkv,Tq", ROWS)
 def test_values_about_zero(kv, dtype, n, H, Hkv, Tq, same):
+    check_mean_zero(kv, dtype, n, H, Hkv, Tq, same)
+
+
+MORE_ROWS = [(4, 2, 5), (8, 2, 5), (2, 2, 16)]         # ten, twenty and sixteen query rows a key/value head
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dh", [8, 40, 64, 96, 128])
+@pytest.mark.parametrize("H,Hkv,Tq", MORE_ROWS)
+def test_a_sentence_of_one_token_is_that_token_in_every_row(kv, dtype, dh, H, Hkv, Tq):
+    check_one_token(kv, dtype, dh, H, Hkv, Tq)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("same", [False, True])
+@pytest.mark.parametrize("n", [3, 100, 2000, 16000])
+@pytest.mark.parametrize("H,Hkv,Tq", MORE_ROWS)
+def test_values_about_zero_in_many_rows(kv, dtype, n, H, Hkv, Tq, same):
     check_mean_zero(kv, dtype, n, H, Hkv, Tq, same)
