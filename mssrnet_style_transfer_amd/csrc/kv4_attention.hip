@@ -11,12 +11,14 @@
 // bf16 scores do not see it; where it counts all codes are 16 times as large, 2^-26, for two shifts more.)
 //
 // What meets the codes is fp16 too (11 bits), as parts whose products add up in fp32: q one part in bf16 calls (exact), two in
-// fp32 ones (2^-22); p s two (2^-22) in either.  One part would keep 2^-12 of the codes'
-// share, which the zeros' share nearly cancels: of a single token's stored values, which come back then, one in five was not the
-// nearest bf16 number, and of values about zero one in three.  Powers of two keep
-// them in fp16's range: a query row is scaled to a largest element in [2^13, 2^14); p s is taken relative to the largest
-// V scale met so far (rounded up to a power of two; when it grows, the sums shrink), with p up to 2^8 (below) and 7 bits
-// on top, so that what is 2^-21 of the largest still has all its bits and the rest is off by at most 2^-32 of it.
+// fp32 ones (2^-22); p s two (2^-22) in either.  One part of p s would keep 2^-12 of the codes' share, which the zeros' share
+// nearly cancels: of a single token's stored values, which come back then, one in five was not the nearest bf16 number, and of
+// values about zero one in three.  Powers of two keep the parts in fp16's range: a query row is scaled to a largest element in
+// [2^13, 2^14) (fp32: [2^9, 2^10); what is 2^-12 of it still has its 22 bits, the rest is off by at most 2^-35 of it).  Every
+// query row and group has its own for p s: the largest met so far lies in [2^6, 2^7) when the unit is chosen and may grow to
+// 2^15 before it is chosen anew (then the sums shrink); what is 2^-9 of it has its 22 bits, the rest is off by at most 2^-31 of it.
+// With one unit for the largest V scale of all rows, groups and tokens, an fp32 result was 3e-3 off where a value 1e6 times as
+// large stood in a token that the row does not attend to.
 //
 // Where values are spread about zero, codes' and zeros' shares of the context nearly cancel, the more so the more tokens
 // there are, and a product's sums are cut, not rounded, where they meet an accumulator that has outgrown them.  7.5 is
@@ -24,8 +26,8 @@
 // tokens starts from zero, added up by rounding additions: fp32 results of 1 .. 16000 tokens of mean zero come out within 1.1e-6
 // in norm, and of bf16 ones 1 or 2 in 1000 are not the nearest number.
 //
-// A wave takes 64 tokens at a time; the running maximum moves only when a score passes it by more than 8 (then every
-// sum is rescaled), so that a block of tokens costs one comparison and no cross-lane reduction.  The W waves of a block
+// A wave takes 64 tokens at a time; a row's running maximum moves only when a score passes it by more than 8, and units of
+// p s only as above (then that row's sums are rescaled), so that a block of tokens costs one comparison and no cross-lane reduction.  The W waves of a block
 // take every W-th 64 tokens of its share of the sentence and are joined through LDS; a second launch joins the shares.
 #include "kv4.hpp"
 
@@ -61,7 +63,9 @@ struct Kv4AttnArgs {
 };
 
 constexpr float KV4_LAZY = 8.f;          // log2 of how far a probability may pass 1 before a rescale
-constexpr float KV4_UP = 7.f;            // log2 of what probabilities are held times
+constexpr int KV4_UP = 7;                // log2 of what the largest p s is held below when its unit is chosen,
+constexpr int KV4_FULL = 15;             // and what it may grow to before the unit is chosen anew
+constexpr int KV4_MOST_UP = 40;          // what no p s is held more than 2^this times: smaller ones are nothing beside the row's sums
 constexpr float KV4_NONE = -3e38f;       // the reference of a row that has seen no token: 2^(-inf - KV4_NONE) is 0
 constexpr float KV4_MID = 7.5f;          // what is taken from codes and added, times the scale, to zeros
 constexpr int KV4_PS_PARTS = 2;          // fp16 parts of p s
@@ -135,12 +139,26 @@ __device__ __forceinline__ void kv4_split(float (&y)[4], f16x8& first, f16x8& se
 // the context cancel: rounded apart, an fp32 result of 1000 tokens was off by 1e-5)
 __device__ __forceinline__ float kv4_pow2(float x) { return __builtin_amdgcn_ldexpf(1.f, (int)fmaxf(x, -512.f)); }
 
-// The exponent of the power of two that bounds the V scales met so far; `top` becomes the largest fp16 number below it, so that
-// a larger scale alone, without a larger power of two, moves nothing.
-__device__ __forceinline__ int kv4_bound(float& top) {
-    const int e = __builtin_amdgcn_frexp_expf(top);
-    top = __builtin_amdgcn_ldexpf(1.f - 0x1p-11f, e);
-    return e;
+// What a row holds a group's p s times, as an exponent: as before (but no more than KV4_MOST_UP) where the largest of the
+// present ones stays below KV4_FULL, else so that it comes to lie in [2^6, 2^7).  most >= 0; by its bits, for the scalar unit.
+__device__ __forceinline__ int kv4_up(int up, float most) {
+    const int e = (int)(__builtin_bit_cast(uint32_t, most) >> 23) - 126;         // most < 2^e
+    up = up < KV4_MOST_UP ? up : KV4_MOST_UP;
+    return e + up > KV4_FULL ? KV4_UP - e : up;
+}
+// 2^x, x <= 0 (nothing below 2^-126)
+__device__ __forceinline__ float kv4_shrink(int x) {
+    return __builtin_bit_cast(float, (uint32_t)(x < -127 ? 0 : x + 127) << 23);
+}
+// the largest of a wave's numbers, none below zero
+__device__ __forceinline__ float kv4_wave_most(float v) {
+    v = fmaxf(v, dpp_mov<0xB1>(v));
+    v = fmaxf(v, dpp_mov<0x4E>(v));
+    v = fmaxf(v, dpp_mov<0x141>(v));
+    v = fmaxf(v, dpp_mov<0x140>(v));
+    v = fmaxf(v, dpp_mov<0x142>(v));             // row_bcast:15, row_bcast:31: the last lane has all
+    v = fmaxf(v, dpp_mov<0x143>(v));
+    return lane_read(v, 63);
 }
 
 // the product of this lane's quad, by two conditions (four nested ones become branches)
@@ -339,7 +357,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
             lim[rr] = k < a.NQ ? (a.causal ? wk.len - (int)a.Tq.d + 1 + ii : wk.len) : 0;
             down[rr] = lane_read(back, rr);
 #pragma unroll
-            for (int g = 0; g < NG; ++g) qsum[rr][g] = lane_read(q.sum[g], rr) * a.scale;
+            for (int g = 0; g < NG; ++g) qsum[rr][g] = lane_read(q.sum[g] * a.scale, rr);
         }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -353,16 +371,21 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
         }
     }
 
-    // m: the running maximum (up to 8 behind), ref: what exponents are taken relative to, ceil(m) - 7 + log2 of the V scales' bound;
-    // every sum of a row is in units of 2^ref, so that nothing but ref remembers either
-    float m[R], ref[R], l[R], zs[R][NG], vtop = 0.f;
+    // m: the running maximum (up to 8 behind), ref: what exponents are taken relative to, ceil(m); l, zs are in units of 2^ref,
+    // a group's codes' share in units of 2^(ref - up)
+    float m[R], ref[R], l[R], zs[R][NG];
+    int up[R][NG];
+    bool fresh = true;
     f32x4 acc[2 * NG];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         m[r] = ref[r] = KV4_NONE;
         l[r] = 0.f;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) zs[r][g] = 0.f;
+        for (int g = 0; g < NG; ++g) {
+            zs[r][g] = 0.f;
+            up[r][g] = KV4_MOST_UP;
+        }
     }
 #pragma unroll
     for (int c = 0; c < 2 * NG; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -382,12 +405,10 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
         const int64_t at = (int64_t)blk * KV4_TOK;
         const bool kept = lane < wk.len - at;
         uint32_t mk[NG], mv[NG];
-        float top = 0.f;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {           // past the sentence's end the cache may hold anything
             mk[g] = kept ? cur.mk[g] : 0u;
             mv[g] = kept ? cur.mv[g] : 0u;
-            top = fmaxf(top, kv4_scale(mv[g]));
         }
         float dot[R], off[R];
 #pragma unroll
@@ -413,7 +434,6 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
         if (more) cur.load_k(ahead, lane, wk.len - at - W * KV4_TOK);
         float s[R];
         uint32_t mask[R];
-        bool far = top > vtop;                   // NaN scales are passed over: they make their own features NaN and no others
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const bool see = lane < lim[r] - at;
@@ -421,41 +441,71 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
             s[r] = see ? s[r] : -INFINITY;
             // one row sees what the sentence has; of several, each may see less, and a NaN that it does not see is not its
             mask[r] = R == 1 || see ? ~0u : 0u;
-            far |= s[r] > m[r] + KV4_LAZY;
         }
-        if (__any(far)) {
-            vtop = fmaxf(vtop, wave_max(top));
-            const float e = vtop > 0.f ? (float)kv4_bound(vtop) - KV4_UP : 0.f;
-            f32x4 f = {1.f, 1.f, 1.f, 1.f};
+        float p[R];
+#pragma unroll 1
+        for (bool move = fresh;; move = true) {
+            if (move) {
+                // Every row for itself, so that no row's rounding depends on its neighbours: its reference, then what its groups'
+                // p s are held times (as much more as p has become less).
+                int rise[R];
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const float top = wave_max(s[r]);
+                    rise[r] = 0;
+                    if (top > m[r] + KV4_LAZY) {
+                        const float moved = ceilf(top), less = kv4_pow2(ref[r] - moved);
+                        rise[r] = __builtin_amdgcn_readfirstlane((int)fminf(moved - ref[r], 512.f));
+                        m[r] = lane_read(top, 0);
+                        ref[r] = lane_read(moved, 0);
+                        l[r] *= less;
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) zs[r][g] *= less;
+                    }
+                    p[r] = __builtin_amdgcn_exp2f(s[r] - ref[r]);
+                }
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    f32x4 f = {1.f, 1.f, 1.f, 1.f};
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        const int next = kv4_up(up[r][g] + rise[r], kv4_wave_most(p[r] * kv4_scale(mv[g] & mask[r])));
+                        f[r] = kv4_shrink(next - up[r][g] - rise[r]);
+                        up[r][g] = next;
+                    }
+                    acc[2 * g] *= f;
+                    acc[2 * g + 1] *= f;
+                }
+            }
+            bool far = false;
+            float big = 0.f;                     // NaN is passed over: it makes its own features NaN and no others
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                m[r] = fmaxf(m[r], wave_max(s[r]));
-                const float moved = ceilf(m[r]) + e;
-                f[r] = kv4_pow2(ref[r] - moved);
-                ref[r] = moved;
-                l[r] *= f[r];
+                far |= s[r] > m[r] + KV4_LAZY;
+                p[r] = __builtin_amdgcn_exp2f(s[r] - ref[r]);
 #pragma unroll
-                for (int g = 0; g < NG; ++g) zs[r][g] *= f[r];
+                for (int g = 0; g < NG; ++g) {
+                    float y = __builtin_amdgcn_ldexpf(p[r] * kv4_scale(mv[g] & mask[r]), up[r][g]);
+                    big = fmaxf(big, y);
+#pragma unroll
+                    for (int part = 0; part < KV4_PS_PARTS; ++part) {
+                        const f16 h = (f16)y;
+                        y -= (float)h;
+                        ps[g][part * R + r][col] = __builtin_bit_cast(uint16_t, h);
+                    }
+                }
             }
-#pragma unroll
-            for (int c = 0; c < 2 * NG; ++c) acc[c] *= f;
+            asm volatile("" ::: "memory");       // (the parts go to LDS here: kept until after the loop they would be spilled)
+            if (move || !__any(far || big > (float)(1 << KV4_FULL))) break;
         }
+        fresh = false;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const float p = __builtin_amdgcn_exp2f(s[r] - ref[r]);
-            l[r] += p;
+            l[r] += p[r];
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 const uint32_t mvr = mv[g] & mask[r];
-                float y = p * kv4_scale(mvr);
-                kv4_pin(y);
-                zs[r][g] = fmaf(p, fmaf(KV4_MID, kv4_scale(mvr), kv4_zero(mvr)), zs[r][g]);
-#pragma unroll
-                for (int part = 0; part < KV4_PS_PARTS; ++part) {
-                    const f16 h = (f16)y;
-                    y -= (float)h;
-                    ps[g][part * R + r][col] = __builtin_bit_cast(uint16_t, h);
-                }
+                zs[r][g] = fmaf(p[r], fmaf(KV4_MID, kv4_scale(mvr), kv4_zero(mvr)), zs[r][g]);
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -492,7 +542,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
         for (int c = 0; c < 2 * NG; ++c) {
             float u = acc[c][r];
             u += __shfl_xor(u, 16);                             // quads 0 and 1
-            u = fmaf(u, 0x1p20f, zt[c >> 1]);
+            u = fmaf(u, __builtin_amdgcn_ldexpf(1.f, 20 - up[r][c >> 1]), zt[c >> 1]);
             if (quad == 0) om[w][r][c * 16 + n] = u;
         }
         if (lane == 0) {
@@ -525,7 +575,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
     constexpr int PARTS = F32 ? 2 : 1;
     constexpr int DP = NG * 32;
     struct Token {
-        float vs[NG][KV4_TOK];              // V scales * 2^-exponent
+        float vs[NG][KV4_TOK];              // V scales
         uint16_t ks[NG][KV4_TOK];           // K scales
         uint2 kz[KV4_TOK];                  // K zeros, groups 0..3
         float vm[NG][KV4_TOK];              // V zeros and KV4_MID V scales
@@ -572,12 +622,14 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
     const float down = __builtin_amdgcn_ldexpf(a.scale, 24 - q.up), downz = __builtin_amdgcn_ldexpf(a.scale, 6 - q.up);
     float m = 0.f;                               // (of no meaning while the row is fresh: it has seen no token yet)
     bool fresh = true;
-    float vtop = 0.f;                            // the largest V scale met; scales are taken times 2^-vexp, which bounds it
-    int vexp = 0;
+    int up[NG];                                  // p s are held times 2^up, the codes' share with them
     f32x4 acc[2 * NG];
     float zs[NG], l = 0.f;                       // of this lane's tokens
 #pragma unroll
-    for (int g = 0; g < NG; ++g) zs[g] = 0.f;
+    for (int g = 0; g < NG; ++g) {
+        zs[g] = 0.f;
+        up[g] = KV4_MOST_UP;
+    }
 #pragma unroll
     for (int c = 0; c < 2 * NG; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
     const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
@@ -619,33 +671,30 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
         float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
 #pragma unroll
         for (int t = 1; t < 4; ++t) top = fmaxf(top, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
-        float big = 0.f;                         // NaN scales are passed over: they make their own features NaN and no others
-#pragma unroll
-        for (int g = 0; g < NG; ++g) big = fmaxf(big, kv4_scale(mv[g]));
-        if (__any(top > KV4_LAZY + KV4_UP || (fresh && top > -INFINITY) || big > vtop)) {
-            vtop = fmaxf(vtop, wave_max(big));
-            const int e = vtop > 0.f ? kv4_bound(vtop) : 0;
-            const float shrink = __builtin_amdgcn_ldexpf(1.f, vexp - e);
-            vexp = e;
+        if (__any(top > KV4_LAZY || (fresh && top > -INFINITY))) {
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
             // by how much this row's reference moves: up, or wherever its first tokens are
-            const float to = ceilf(top - KV4_UP);
-            const float up = !fresh ? fmaxf(to, 0.f) : top > -INFINITY ? to : 0.f;
-            const float f = fresh ? 1.f : kv4_pow2(-up);
-            fresh = fresh && !(top > -INFINITY);
-            m += up;
-            l *= f;
+            const bool moves = fresh ? top > -INFINITY : top > KV4_LAZY;
+            const float by = moves ? ceilf(top) : 0.f, less = fresh ? 1.f : kv4_pow2(-by);
+            const int rise = fresh ? 0 : (int)fminf(by, 512.f);
+            fresh = fresh && !moves;
+            m += by;
+            l *= less;
 #pragma unroll
-            for (int g = 0; g < NG; ++g) zs[g] *= f;
-#pragma unroll
-            for (int c = 0; c < 2 * NG; ++c) acc[c] *= f * shrink;
+            for (int g = 0; g < NG; ++g) {
+                zs[g] *= less;
+                const int next = up[g] + rise < KV4_MOST_UP ? up[g] + rise : KV4_MOST_UP;
+                const float f = kv4_shrink(next - up[g] - rise);
+                up[g] = next;
+                acc[2 * g] *= f;
+                acc[2 * g + 1] *= f;
+            }
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[t][r] -= up;
+                for (int r = 0; r < 4; ++r) s[t][r] -= by;
         }
-        const float vmul = __builtin_amdgcn_ldexpf(1.f, -vexp);
         bool nan = false;
 #pragma unroll
         for (int g = 0; g < NG; ++g) nan |= kv4_scale(mv[g]) != kv4_scale(mv[g]);
@@ -653,7 +702,7 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             const float vz = kv4_zero(mv[g]);
-            my.vs[g][lane] = kv4_scale(mv[g]) * vmul;
+            my.vs[g][lane] = kv4_scale(mv[g]);
             my.vm[g][lane] = vz == vz ? fmaf(KV4_MID, kv4_scale(mv[g]), vz) : 0.f;
         }
         __builtin_amdgcn_wave_barrier();
@@ -672,22 +721,37 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
             f32x4 c[PARTS][2], mid = zero4;
 #pragma unroll
             for (int part = 0; part < PARTS; ++part) c[part][0] = c[part][1] = zero4;
+            float y[4][4], most = 0.f;           // NaN scales are passed over: they make their own features NaN and no others
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const f32x4 v4 = *reinterpret_cast<const f32x4*>(&my.vs[g][16 * t + 4 * quad]);
+                const f32x4 z4 = *reinterpret_cast<const f32x4*>(&my.vm[g][16 * t + 4 * quad]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    zs[g] = fmaf(s[t][r], z4[r], zs[g]);
+                    y[t][r] = s[t][r] * v4[r];
+                    if (__builtin_expect(hidden, 0)) y[t][r] = 16 * t + 4 * quad + r < see ? y[t][r] : 0.f;
+                    most = fmaxf(most, y[t][r]);
+                }
+            }
+            if (__any(__builtin_amdgcn_ldexpf(most, up[g]) > (float)(1 << KV4_FULL))) {
+                most = fmaxf(most, __shfl_xor(most, 16));
+                most = fmaxf(most, __shfl_xor(most, 32));
+                const int next = kv4_up(up[g], most);
+                const float f = kv4_shrink(next - up[g]);
+                up[g] = next;
+                acc[2 * g] *= f;
+                acc[2 * g + 1] *= f;
+            }
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
                 f16x8 pop[KV4_PS_PARTS];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int t = 2 * ks + h;
-                    const f32x4 v4 = *reinterpret_cast<const f32x4*>(&my.vs[g][16 * t + 4 * quad]);
-                    const f32x4 z4 = *reinterpret_cast<const f32x4*>(&my.vm[g][16 * t + 4 * quad]);
-                    float y[4];
+                    float (&part)[4] = y[2 * ks + h];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        zs[g] = fmaf(s[t][r], z4[r], zs[g]);
-                        y[r] = s[t][r] * v4[r];
-                        if (__builtin_expect(hidden, 0)) y[r] = 16 * t + 4 * quad + r < see ? y[r] : 0.f;
-                    }
-                    kv4_split<F32>(y, pop[0], pop[1], h);
+                    for (int r = 0; r < 4; ++r) part[r] = __builtin_amdgcn_ldexpf(part[r], up[g]);
+                    kv4_split<F32>(part, pop[0], pop[1], h);
                 }
                 const int d = (ks * NG + g) * 2;
                 f16x8 lo, hi;
@@ -732,11 +796,11 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
         if (more) cur.load_v(ahead, lane);
     }
 
-    const float unit = __builtin_amdgcn_ldexpf(1.f, 20 + vexp);
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
+        const float unit = __builtin_amdgcn_ldexpf(1.f, 20 - up[g]);
         float z = zs[g];
         z += __shfl_xor(z, 16);
         z += __shfl_xor(z, 32);

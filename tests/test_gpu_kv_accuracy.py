@@ -108,3 +108,82 @@ def test_a_sentence_of_one_token_is_that_token_in_every_row(kv, dtype, dh, H, Hk
 @pytest.mark.parametrize("H,Hkv,Tq", MORE_ROWS)
 def test_values_about_zero_in_many_rows(kv, dtype, n, H, Hkv, Tq, same):
     check_mean_zero(kv, dtype, n, H, Hkv, Tq, same)
+
+
+# ------------------------------------------------------------------------------------------------ values of other sizes beside
+ALL_ROWS = ROWS + MORE_ROWS
+# p s is held to 2^-22 of itself, its products and sums in fp32: 4 deviations * 2^-21 = 2e-6 as in check_mean_zero; the largest of
+# some 50 rows' errors is twice the typical one.  The scores' part is small: keys of deviation 1 and queries of 1.
+BESIDE = 5e-6
+
+
+def judge_rows(got, want, share):
+    """judge() of every query row and group of 32 features for itself."""
+    for a, b in zip(got.split(32, -1), want.split(32, -1)):
+        if got.dtype == torch.float32:
+            err = ((a.double() - b).norm(dim=-1) / b.norm(dim=-1)).max()
+            assert float(err) <= share + 2.0 ** -24, "%.3g of a row, %.3g allowed" % (float(err), share)
+        else:
+            judge(a, b, 2 * share)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("ratio", [1e3, 1e6])
+@pytest.mark.parametrize("where", [2, 150, 299])
+@pytest.mark.parametrize("H,Hkv,Tq", ALL_ROWS)
+def test_a_large_value_that_nobody_attends_to(kv, dtype, ratio, where, H, Hkv, Tq):
+    B, n, dh = 3, 300, 64
+    k, v, q = heads(B, Hkv, n, dh, dtype, 21), heads(B, Hkv, n, dh, dtype, 22), heads(B, H, Tq, dh, dtype, 23)
+    q[..., 0] = 8.0                                     # the token's key is far off along this feature for every row
+    k[..., 0] *= 0.01
+    k[:, :, where, 0] = -100.0
+    v *= 1e-3
+    v[:, :, where] *= ratio
+    c = kv.KVCache4(B, Hkv, dh, n)
+    c.write(k, v)
+    want = exact(q, values(k), values(v), 1 / math.sqrt(dh))
+    judge_rows(kv.attention(q, c, n), want, BESIDE)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,Hkv,Tq", [r for r in ALL_ROWS if r[0] * r[2] > r[1]])
+def test_a_large_value_that_one_row_attends_to(kv, dtype, H, Hkv, Tq):
+    B, n, dh = 2, 200, 64
+    k, v, q = heads(B, Hkv, n, dh, dtype, 31), heads(B, Hkv, n, dh, dtype, 32), heads(B, H, Tq, dh, dtype, 33)
+    q[..., 0] = 8.0
+    q[:, ::H // Hkv, 0, 0] = -8.0                       # the first row of every key/value head
+    k[..., 0] *= 0.01
+    k[:, :, 70, 0] = -100.0
+    v *= 1e-3
+    v[:, :, 70] *= 1e6
+    c = kv.KVCache4(B, Hkv, dh, n)
+    c.write(k, v)
+    want = exact(q, values(k), values(v), 1 / math.sqrt(dh))
+    assert (want[:, 0, 0].abs().amax(-1) > 100).all() and (want[:, 0, 1:] if Tq > 1 else want[:, 1]).abs().max() < 1e-2
+    judge_rows(kv.attention(q, c, n), want, BESIDE)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,Hkv,Tq", ALL_ROWS)
+def test_groups_of_other_sizes(kv, dtype, H, Hkv, Tq):
+    B, n, dh = 3, 500, 96
+    k, v, q = heads(B, Hkv, n, dh, dtype, 41), heads(B, Hkv, n, dh, dtype, 42), heads(B, H, Tq, dh, dtype, 43)
+    v[..., :32] *= 1e3
+    v[..., 64:] *= 1e-3
+    c = kv.KVCache4(B, Hkv, dh, n)
+    c.write(k, v)
+    judge_rows(kv.attention(q, c, n), exact(q, values(k), values(v), 1 / math.sqrt(dh)), BESIDE)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,Hkv,Tq", [(4, 2, 2), (4, 2, 5), (2, 2, 16)])
+def test_a_large_value_that_later_rows_see(kv, dtype, H, Hkv, Tq):
+    B, n, dh = 2, 130, 64
+    k, v, q = heads(B, Hkv, n, dh, dtype, 51), heads(B, Hkv, n, dh, dtype, 52), heads(B, H, Tq, dh, dtype, 53)
+    v *= 1e-3
+    v[:, :, n - 1] *= 1e6
+    c = kv.KVCache4(B, Hkv, dh, n)
+    c.write(k, v)
+    see = torch.arange(n, device="cuda") < (n - Tq + 1 + torch.arange(Tq, device="cuda")).view(1, Tq, 1)
+    want = exact(q, values(k), values(v), 1 / math.sqrt(dh), see.expand(B, Tq, n))
+    judge_rows(kv.attention(q, c, n, causal=True), want, BESIDE)
