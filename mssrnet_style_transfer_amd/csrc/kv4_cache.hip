@@ -43,8 +43,9 @@ __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
 // The group's codes of this lane's 8 features (one byte each, features 0-3 in c0, 4-7 in c1) and its (s, z) word.
 // `live`: the lane holds features (a head's last group may have fewer than 32).  All four lanes of a group call it.
 // Bound by vector instructions as soon as memory is not waited for, hence: minima and maxima three at a time, NaN two at a
-// time, infinities by the extremes, no clamp of the elements (codes are clamped, and x beyond the clamped extremes has the
-// extreme's code), conversion and packing in one instruction.
+// time, infinities by the extremes, the elements' clamp by their codes' (x - z, its product with 1/s and its rounding keep order:
+// what lies below -65504 has code 0 as -65504 has, what lies above 65504 at most the code of 65504), conversion and packing in
+// one instruction.
 __device__ __forceinline__ void kv4_quantise(const float (&x)[8], bool live, uint32_t& c0, uint32_t& c1, uint32_t& meta) {
 #pragma clang fp contract(off)
     float lo = fminf(fminf(fminf(fminf(x[0], x[1]), x[2]), fminf(fminf(x[3], x[4]), x[5])), fminf(x[6], x[7]));
@@ -72,10 +73,11 @@ __device__ __forceinline__ void kv4_quantise(const float (&x)[8], bool live, uin
     // 1 / s, correctly rounded: one Newton step from the hardware's estimate, checked for every positive fp16 number
     const float r0 = __builtin_amdgcn_rcpf(sf);
     const float inv = sf > 0.f ? __builtin_fmaf(__builtin_fmaf(-sf, r0, 1.f), r0, r0) : 0.f;
+    const float most = fminf((65504.f - zf) * inv, 15.f);
     c0 = c1 = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float q = __builtin_rintf(__builtin_amdgcn_fmed3f((x[i] - zf) * inv, 0.f, 15.f));
+        const float q = __builtin_rintf(__builtin_amdgcn_fmed3f((x[i] - zf) * inv, 0.f, most));
         if (i < 4) c0 = __builtin_amdgcn_cvt_pk_u8_f32(q, i, c0);
         else c1 = __builtin_amdgcn_cvt_pk_u8_f32(q, i - 4, c1);
     }

@@ -541,3 +541,18 @@ def test_longest_shapes_the_launch_and_nothing_else(kv, longest):
         n = torch.tensor([3000, 1234], device="cuda")
         want, bound = attend(q, values(k), values(v), n, 1 / 8, False)
         close(kv.attention(q, c, n, longest=longest), want, bound, "longest %d" % longest)
+
+
+@pytest.mark.parametrize("T,B", [(6, 1), (64, 140)])                # token by token, and whole blocks
+def test_values_beyond_the_clamp_in_a_group_that_reaches_it(kv, T, B):
+    # the group's range ends at the clamp and is narrow: codes of 65504 and of what lies beyond it would differ
+    x = torch.zeros(B, 8, T, 64, device="cuda")
+    for t, base in enumerate((65490.0, 65500.0, 65400.0, 60000.0, 65504.0, 65488.0)):
+        x[:, :, t] = base
+        x[:, :, t, 7], x[:, :, t, 40:44] = 1e6, 3e38
+        x[:, :, t, 50] = base - 30.0
+    x[:, 4:] *= -1
+    c = kv.KVCache4(B, 8, 64, T)
+    c.write(x, x)
+    for got in c.read(0, T):
+        assert torch.equal(got, values(x).float())
