@@ -14,7 +14,7 @@
 // fp32 ones (2^-22); p s two (2^-22) in either.  One part of p s would keep 2^-12 of the codes' share, which the zeros' share
 // nearly cancels: of a single token's stored values, which come back then, one in five was not the nearest bf16 number, and of
 // values about zero one in three.  Powers of two keep the parts in fp16's range: a query row is scaled to a largest element in
-// [2^13, 2^14) (fp32: [2^9, 2^10); what is 2^-12 of it still has its 22 bits, the rest is off by at most 2^-35 of it).  Every
+// [2^13, 2^14) (fp32: [2^9, 2^10); what is 2^-11 of it still has its 22 bits, the rest is off by at most 2^-34 of it).  Every
 // query row and group has its own for p s: the largest met so far lies in [2^6, 2^7) when the unit is chosen and may grow to
 // 2^15 before it is chosen anew (then the sums shrink); what is 2^-9 of it has its 22 bits, the rest is off by at most 2^-31 of it.
 // With one unit for the largest V scale of all rows, groups and tokens, an fp32 result was 3e-3 off where a value 1e6 times as
@@ -33,8 +33,8 @@
 
 namespace mssr {
 
-// Division of a number below 2^31 by one the host knows: a high product, an addition, a shift
-// (m = floor(2^32 (2^shift - d) / d) + 1, shift = ceil(log2 d)).
+// Division of a number below 2^31 by one the host knows: a high product, an addition, a shift (Granlund and Montgomery,
+// "Division by Invariant Integers using Multiplication", 1994; m = floor(2^32 (2^shift - d) / d) + 1, shift = ceil(log2 d)).
 struct Divisor {
     uint32_t d, m, shift;
     Divisor() = default;
