@@ -9,6 +9,7 @@ import struct
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int64, c_uint64, c_void_p
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libmssr_hip.so")
@@ -280,6 +281,20 @@ def stream():
 def raw_stream(index):
     """The current stream of device ``index`` as stream() gives it, without building a torch.cuda.Stream (2.7 us a call)."""
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+def refuse_graph(who, *tensors):
+    """For operators without a backward: raises where a result would need a graph or a forward-mode tangent (which
+    torch.no_grad() does not turn off).  Arguments that are no tensors are passed over."""
+    grad, tangents = torch.is_grad_enabled(), forward_ad._current_level >= 0
+    if not grad and not tangents:
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor):
+            if grad and t.requires_grad:
+                raise RuntimeError("%s builds no graph: call it under torch.no_grad()" % who)
+            if tangents and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("%s builds no graph: call it on tensors without tangents" % who)
 
 
 def require_cuda(*tensors):

@@ -5,7 +5,7 @@ memory_values``) of a decoder layer's cache (onmt/decoders/transformer.py:268-28
 131-160): every 32 features of a token and head are 4-bit codes with an fp16 scale and zero, 5 bits a feature where the
 reference keeps 32.  Tokens are quantised once, when they are written; ``attention`` multiplies the codes as they lie.
 
-These are decoding operators: they build no graph and refuse inputs that would need one.
+These are decoding operators: they build no graph and refuse inputs that would need one, or that carry a forward-mode tangent.
 """
 import ctypes
 from functools import lru_cache
@@ -19,10 +19,6 @@ MAX_DIM = 128
 
 _INTS = (torch.int32, torch.int64)
 _pack_rows, _pack_attention = L.packer(L.Kv4Rows), L.packer(L.Kv4AttentionDesc)
-
-
-def _needs_graph(who):
-    raise RuntimeError("%s builds no graph: call it under torch.no_grad()" % who)
 
 
 def _index(who, name, t, B, device):
@@ -113,8 +109,7 @@ class KVCache4:
         ``start`` is a tensor and refused where it is an int.  A group of 32 features that holds a NaN or an infinity reads
         back as NaN; values beyond +-65504 are clamped to that."""
         who = "KVCache4.write"
-        if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
-            _needs_graph(who)
+        L.refuse_graph(who, k, v)
         if not (k.is_cuda and v.is_cuda):
             L.require_cuda(k, v)
         k, v = self._rows(who, "k", k), self._rows(who, "v", v)
@@ -165,8 +160,7 @@ def attention(q, cache, lengths, scale=None, causal=False, longest=0):
     capacity (it shapes the launch, nothing else).  Returns [B, H, T, dim], a view of [B, T, H, dim] memory, in q's type;
     probabilities are not returned."""
     who = "kv_cache.attention"
-    if q.requires_grad and torch.is_grad_enabled():
-        _needs_graph(who)
+    L.refuse_graph(who, q)
     if not q.is_cuda:
         L.require_cuda(q)
     device, shape, dh = cache.device, q.shape, cache.dim

@@ -2,7 +2,8 @@
 
 What stands between a decoder's generator and its pick (the reference's search takes the largest logit,
 onmt/translate/greedy_search.py:135-165, with its n-gram rule in onmt/translate/decode_strategy.py): one pass over the
-logits, which leaves either new logits (for a sampler) or only the picked ids.  Decoding operators: they build no graph.
+logits, which leaves either new logits (for a sampler) or only the picked ids.  Decoding operators: they build no graph and
+refuse logits, biases and rates that would need one, or that carry a forward-mode tangent.
 """
 from dataclasses import dataclass
 from functools import lru_cache
@@ -96,8 +97,8 @@ def _address(t):
 
 def _call(who, logits, control, history, lengths, prompt_lengths, out, ids, empty):
     """Checks, then one call; every tensor made on the way is a local and lives until it is launched."""
-    if logits.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("%s builds no graph: call it under torch.no_grad()" % who)
+    c = _NO_RULES if control is None else control
+    L.refuse_graph(who, logits, c.bias, c.repetition, c.frequency, c.presence, out)
     if not logits.is_cuda:
         L.require_cuda(logits)
     if logits.dim() != 2 or logits.shape[1] == 0:
@@ -106,7 +107,6 @@ def _call(who, logits, control, history, lengths, prompt_lengths, out, ids, empt
     dev = logits.device
     if not logits.is_contiguous() and (V > 1 and logits.stride(1) != 1 or B > 1 and logits.stride(0) < V):
         logits = logits.contiguous()
-    c = _NO_RULES if control is None else control
     bits = h_bs = h_ts = T = bias_bs = states = mode = 0
     if history is not None:
         if not isinstance(history, torch.Tensor) or history.dim() != 2 or history.shape[0] != B or \

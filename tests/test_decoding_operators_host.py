@@ -153,3 +153,38 @@ def test_cpu_tensors_are_refused():
         token_control.pick_token(torch.zeros(2, 5))
     with pytest.raises(ValueError):
         kv_cache.KVCache4(1, 1, 60, 4, device="cpu")
+
+
+def without_gpu(fn, *args, **kw):
+    """What a call says on CPU tensors: graphs are refused before devices."""
+    with pytest.raises(RuntimeError) as e:
+        fn(*args, **kw)
+    return str(e.value)
+
+
+def test_graphs_and_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+
+    from mssrnet_style_transfer_amd import kv_cache, token_control
+    x, h, n = torch.ones(2, 5), torch.zeros(2, 2, 1, 64), torch.ones(2)
+    cache = kv_cache.KVCache4.__new__(kv_cache.KVCache4)
+
+    def calls(mark):
+        yield kv_cache.attention, (mark(h), cache, 1), {}
+        yield cache.write, (mark(h), h), {}
+        yield cache.write, (h, mark(h)), {}
+        for fn in (token_control.pick_token, token_control.control_logits):
+            yield fn, (mark(x),), {}
+            for name, t in (("bias", x), ("repetition", n), ("frequency", n), ("presence", n)):
+                yield fn, (x, TokenControl(**{name: mark(t)})), {}
+        yield token_control.control_logits, (x,), dict(out=mark(x.clone()))
+
+    for fn, args, kw in calls(lambda t: t.clone().requires_grad_()):
+        assert "no graph" in without_gpu(fn, *args, **kw)
+        with torch.no_grad():                       # then they are the data that they are
+            assert "no CPU path" in without_gpu(fn, *args, **kw)
+    with fwd.dual_level():
+        for fn, args, kw in calls(lambda t: fwd.make_dual(t.clone(), t.clone())):
+            with torch.no_grad():
+                assert "without tangents" in without_gpu(fn, *args, **kw)
+        assert "no CPU path" in without_gpu(token_control.pick_token, x, TokenControl(bias=x))
