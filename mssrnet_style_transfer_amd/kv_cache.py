@@ -75,12 +75,14 @@ class KVCache4:
         return dict(self.__dict__, _held=None)      # checkpoints and copies hold the data, not its address
 
     def _desc(self):
-        """The address of the C descriptor of the present data (built again where that has moved or changed its batch)."""
-        at = (self.data.data_ptr(), self.data.shape[0])
-        if self._held is None or self._held[0] != at:
+        """(what it describes, the C descriptor of the present data, its address), built again where the data has moved or
+        changed its batch.  A caller keeps the tuple until its C call is over: another thread may have replaced it here by
+        then, and the address alone keeps nothing alive."""
+        at, held = (self.data.data_ptr(), self.data.shape[0]), self._held
+        if held is None or held[0] != at:
             d = L.Kv4Cache(*at, self.capacity, self.heads, self.dim)
-            self._held = (at, d, ctypes.addressof(d))
-        return self._held[2]
+            self._held = held = (at, d, ctypes.addressof(d))
+        return held
 
     def _span(self, who, start, T, counts):
         B, device = self.batch, self.device
@@ -122,8 +124,9 @@ class KVCache4:
             return
         kb, kh, kt, _ = k.stride()
         vb, vh, vt, _ = v.stride()
+        held = self._desc()
         L.call("mssr_kv4_write", device, _pack_rows(
-            self._desc(), k.data_ptr(), kb, kh, kt, v.data_ptr(), vb, vh, vt, T, _address(start), start0, _address(counts),
+            held[2], k.data_ptr(), kb, kh, kt, v.data_ptr(), vb, vh, vt, T, _address(start), start0, _address(counts),
             bits, L.dt(k)))
 
     def read(self, start, length, counts=None, dtype=torch.float32):
@@ -140,8 +143,9 @@ class KVCache4:
         k, v = both.unbind(0)
         if B == 0:
             return k, v
+        held = self._desc()
         L.call("mssr_kv4_read", self.device, _pack_rows(
-            self._desc(), k.data_ptr(), T * H * dh, dh, H * dh, v.data_ptr(), T * H * dh, dh, H * dh, T, _address(start),
+            held[2], k.data_ptr(), T * H * dh, dh, H * dh, v.data_ptr(), T * H * dh, dh, H * dh, T, _address(start),
             start0, _address(counts), bits, L.dt(k)))
         return k, v
 
@@ -184,7 +188,8 @@ def attention(q, cache, lengths, scale=None, causal=False, longest=0):
     # from the allocator, per call: a call's scratch is its own on every stream and in every captured graph
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
     qb, qh, qt, _ = q.stride()
+    held = cache._desc()
     L.call("mssr_kv4_attention", device, _pack_attention(
-        cache._desc(), q.data_ptr(), qb, qh, qt, out.data_ptr(), T * H * dh, dh, H * dh, T, _address(lengths), n, longest,
+        held[2], q.data_ptr(), qb, qh, qt, out.data_ptr(), T * H * dh, dh, H * dh, T, _address(lengths), n, longest,
         _address(ws), need, H, wide, dh ** -0.5 if scale is None else scale, 1 if causal else 0, code))
     return out

@@ -188,3 +188,42 @@ def test_graphs_and_tangents_are_refused():
             with torch.no_grad():
                 assert "without tangents" in without_gpu(fn, *args, **kw)
         assert "no CPU path" in without_gpu(token_control.pick_token, x, TokenControl(bias=x))
+
+
+def test_a_descriptor_lives_until_its_call_is_over(monkeypatch):
+    """Two threads' first calls on one cache both build its descriptor, and the second replaces the first while that one's C
+    call may read it.  Here the other thread's turn comes inside the call, by hand."""
+    import struct
+    import weakref
+
+    from mssrnet_style_transfer_amd import kv_cache
+    made = []
+
+    class Watched(L.Kv4Cache):
+        def __init__(self, *args):
+            super().__init__(*args)
+            made.append((ctypes.addressof(self), weakref.ref(self)))
+
+    class OnDevice(torch.Tensor):               # CPU data that passes for a device's
+        is_cuda = True
+
+    calls = []
+
+    def call(name, device, desc):
+        address = struct.unpack_from("P", desc)[0]
+        other = L.Kv4Cache(0, 2, 64, 2, 64)         # the other thread found none either, built its own
+        cache._held = (None, other, 0)              # and stores it
+        assert any(a == address and ref() is not None for a, ref in made), name
+        calls.append(name)
+
+    monkeypatch.setattr(L, "Kv4Cache", Watched)
+    monkeypatch.setattr(L, "call", call)
+    monkeypatch.setattr(kv_cache, "_scratch_bytes", lambda *a: 0)
+    cache = kv_cache.KVCache4.__new__(kv_cache.KVCache4)
+    cache.heads, cache.dim, cache.capacity, cache._held = 2, 64, 64, None
+    cache.data = torch.zeros(2, L.load().mssr_kv4_bytes(2, 2, 64, 64) // 2, dtype=torch.uint8)
+    x = torch.zeros(2, 2, 1, 64).as_subclass(OnDevice)
+    for fn in (lambda: cache.write(x, x), lambda: cache.read(0, 1), lambda: kv_cache.attention(x, cache, 1)):
+        cache._held = None
+        fn()
+    assert calls == ["mssr_kv4_write", "mssr_kv4_read", "mssr_kv4_attention"]
