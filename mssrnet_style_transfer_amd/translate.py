@@ -19,37 +19,46 @@ def greedy_decode_cached(model, cfg, memory_bank, src_lengths, max_length, kv_bi
     past a sentence's first </s> unspecified."""
     dev, B = memory_bank.device, memory_bank.size(1)
     src_lengths = src_lengths.to(dev)
-    lin = model.generator[0]
+    if max_length == 0:
+        return torch.empty(0, B, dtype=torch.int32, device=dev)
     with torch.no_grad():
         src = torch.zeros(memory_bank.size(0), B, 1, dtype=torch.long, device=dev)
         model.decoder.init_state(src, memory_bank, None, kv_bits=kv_bits, max_steps=max_length)
-        out = torch.full((max_length, B), cfg.eos_idx, dtype=torch.int32, device=dev)
-        ids = torch.full((max_length, B), cfg.eos_idx, dtype=torch.int32, device=dev)     # columns of the running sentences
-        rows = torch.arange(B, device=dev)
-        tok = torch.full((1, B, 1), cfg.bos_idx, dtype=torch.long, device=dev)
-        done = torch.zeros(B, dtype=torch.bool, device=dev)
-        flushed = steps = 0
-        for step in range(max_length):
-            dec_out, _ = model.decoder(tok, memory_bank, memory_lengths=src_lengths, step=step)
-            logits = ops.linear(dec_out[-1], lin.weight, lin.bias)
-            pick_token(logits, control, ids[:step].t() if step else None, empty=cfg.eos_idx, out=ids[step])
-            tok = ids[step].long().view(1, -1, 1)
-            steps = step + 1
-            if steps % check_every and steps != max_length:
-                continue
-            out[flushed:steps, rows] = ids[flushed:steps]
-            done[rows] |= (ids[flushed:steps] == cfg.eos_idx).any(0)
-            flushed = steps
-            keep = (~done[rows]).nonzero().squeeze(1)       # the one host sync of this check point
-            if keep.numel() == 0 or steps == max_length:
-                break
-            if keep.numel() < rows.numel():
-                model.decoder.map_state(lambda t, dim: t.index_select(dim, keep))
-                memory_bank, src_lengths = memory_bank.index_select(1, keep), src_lengths.index_select(0, keep)
-                if control is not None:
-                    control = control.rows(keep, rows.numel())
-                tok, ids, rows = tok.index_select(1, keep), ids.index_select(1, keep), rows.index_select(0, keep)
-        model.decoder.init_state(None, None, None)          # the cache goes with the search, not into the next checkpoint
+        try:
+            return _cached_steps(model, cfg, memory_bank, src_lengths, max_length, control, check_every)
+        finally:                                            # the cache goes with the search, not into the next checkpoint
+            model.decoder.init_state(None, None, None)
+
+
+def _cached_steps(model, cfg, memory_bank, src_lengths, max_length, control, check_every):
+    """The steps of greedy_decode_cached over the decoder's state."""
+    dev, B, lin = memory_bank.device, memory_bank.size(1), model.generator[0]
+    out = torch.full((max_length, B), cfg.eos_idx, dtype=torch.int32, device=dev)
+    ids = torch.full((max_length, B), cfg.eos_idx, dtype=torch.int32, device=dev)     # columns of the running sentences
+    rows = torch.arange(B, device=dev)
+    tok = torch.full((1, B, 1), cfg.bos_idx, dtype=torch.long, device=dev)
+    done = torch.zeros(B, dtype=torch.bool, device=dev)
+    flushed = steps = 0
+    for step in range(max_length):
+        dec_out, _ = model.decoder(tok, memory_bank, memory_lengths=src_lengths, step=step)
+        logits = ops.linear(dec_out[-1], lin.weight, lin.bias)
+        pick_token(logits, control, ids[:step].t() if step else None, empty=cfg.eos_idx, out=ids[step])
+        tok = ids[step].long().view(1, -1, 1)
+        steps = step + 1
+        if steps % check_every and steps != max_length:
+            continue
+        out[flushed:steps, rows] = ids[flushed:steps]
+        done[rows] |= (ids[flushed:steps] == cfg.eos_idx).any(0)
+        flushed = steps
+        keep = (~done[rows]).nonzero().squeeze(1)       # the one host sync of this check point
+        if keep.numel() == 0 or steps == max_length:
+            break
+        if keep.numel() < rows.numel():
+            model.decoder.map_state(lambda t, dim: t.index_select(dim, keep))
+            memory_bank, src_lengths = memory_bank.index_select(1, keep), src_lengths.index_select(0, keep)
+            if control is not None:
+                control = control.rows(keep, rows.numel())
+            tok, ids, rows = tok.index_select(1, keep), ids.index_select(1, keep), rows.index_select(0, keep)
     return out[:steps]
 
 

@@ -227,3 +227,19 @@ def test_a_descriptor_lives_until_its_call_is_over(monkeypatch):
         cache._held = None
         fn()
     assert calls == ["mssr_kv4_write", "mssr_kv4_read", "mssr_kv4_attention"]
+
+
+def test_a_cached_search_that_fails_leaves_no_state():
+    from types import SimpleNamespace
+
+    from mssrnet_style_transfer_amd.config import MSSRConfig
+    from mssrnet_style_transfer_amd.style_generator_builder import build_all
+    from mssrnet_style_transfer_amd.translate import greedy_decode_cached
+    cfg = MSSRConfig.small()
+    model = build_all(cfg, device="cpu", seed=1)["model"].eval()
+    mem, lens = torch.zeros(5, 3, cfg.d_model), torch.tensor([5, 2, 3])
+    with pytest.raises(RuntimeError, match="no CPU path"):              # the first step's cache has no place on the CPU
+        greedy_decode_cached(model, cfg, mem, lens, 4)
+    assert all(model.decoder.state[name] is None for name in ("src", "cache", "kv4_steps"))
+    nothing = SimpleNamespace()                                         # a search of no steps asks nothing of the model
+    assert greedy_decode_cached(nothing, cfg, mem, lens, 0).shape == (0, 3)

@@ -224,3 +224,14 @@ def test_a_4bit_state_is_cut_down_and_refused(ops):
     dec.init_state(src, mem, None, kv_bits=4, max_steps=4)
     with pytest.raises(RuntimeError, match="no graph"):                  # outside no_grad
         dec(tokens[0].view(1, 5, 1), mem, memory_lengths=lens, step=0)
+
+
+def test_a_cached_search_whose_rules_do_not_fit_leaves_no_state(ops):
+    from mssrnet_style_transfer_amd import token_control as tc
+    from mssrnet_style_transfer_amd.translate import greedy_decode_cached
+    cfg, nets, mem, lens = setup(B=4)
+    decoder = nets["model"].decoder
+    with pytest.raises(ValueError, match="bias"):                       # noticed after the first step has filled its caches
+        greedy_decode_cached(nets["model"], cfg, mem, lens, 6, control=tc.TokenControl(bias=torch.zeros(3, device="cuda")))
+    assert all(decoder.state[name] is None for name in ("src", "cache", "kv4_steps"))
+    assert greedy_decode_cached(nets["model"], cfg, mem, lens, 0).shape == (0, 4)
