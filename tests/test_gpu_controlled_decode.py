@@ -235,3 +235,49 @@ def test_a_cached_search_whose_rules_do_not_fit_leaves_no_state(ops):
         greedy_decode_cached(nets["model"], cfg, mem, lens, 6, control=tc.TokenControl(bias=torch.zeros(3, device="cuda")))
     assert all(decoder.state[name] is None for name in ("src", "cache", "kv4_steps"))
     assert greedy_decode_cached(nets["model"], cfg, mem, lens, 0).shape == (0, 4)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_controlled_sentences_leave_the_batch(ops, dtype, monkeypatch):
+    """Rules of every kind a row can have, in a search that drops finished sentences again and again, against the host's and
+    against the same search that drops none."""
+    from mssrnet_style_transfer_amd import token_control as tc
+    from mssrnet_style_transfer_amd.decode_engine import greedy_decode_ids
+    B, T = 40, 20
+    cuts = []
+    rows = tc.TokenControl.rows
+    monkeypatch.setattr(tc.TokenControl, "rows", lambda self, index, batch: cuts.append(batch) or rows(self, index, batch))
+    ops.set_compute_dtype(dtype)
+    try:
+        cfg, nets, mem, lens = setup(B=B)
+        model, V = nets["model"], cfg.vocab_size
+        g = torch.Generator(device="cuda").manual_seed(5)
+        # each sentence has its own order of words, a step of 1 apart (no word twice: it goes down the list), </s> at its own place
+        bias = torch.rand(B, V, device="cuda", generator=g).argsort(1).float() - V
+        place = torch.arange(B, device="cuda") % 16
+        bias[:, cfg.eos_idx] = -(place + 0.5)
+        bits = torch.rand(4, V, device="cuda", generator=g) < 0.8
+        bits[:, cfg.eos_idx] = True
+        control = tc.TokenControl(repetition=1 + torch.rand(B, device="cuda", generator=g), frequency=0.1,
+                                  presence=torch.rand(B, device="cuda", generator=g), ngram=1, bias=bias,
+                                  allowed=tc.pack_allowed(bits), state=torch.randint(-1, 4, (B,), device="cuda", generator=g))
+        with torch.no_grad():
+            want, margin, top = reference_steps(ops, model, cfg, mem, lens, control, bits, T)
+            never = greedy_decode_ids(model, cfg, mem, lens, T, control=control, compact_below=0.0).cpu()
+            assert not cuts
+            got = greedy_decode_ids(model, cfg, mem, lens, T, control=control, check_every=2, compact_below=0.99).cpu()
+    finally:
+        ops.set_compute_dtype(torch.float32)
+    assert len(cuts) >= 2 and cuts == sorted(cuts, reverse=True) and cuts[0] == B, cuts
+    close = 4 * top * (1e-4 if dtype == torch.float32 else 2e-2)         # as in test_controlled_greedy_decode
+    agreed = total = 0
+    for b in range(B):
+        n = first_end(want[:, b].tolist(), cfg.eos_idx)
+        total += n
+        for t in range(n):
+            if margin[t, b] < close:
+                break
+            assert int(got[t, b]) == int(never[t, b]) == int(want[t, b]), (b, t)
+            agreed += 1
+    # words are a step of 1 apart, logits spread by `top`: a margin is below `close` for about that share of the words
+    assert agreed >= (0.9 if dtype == torch.float32 else 0.5) * total, (agreed, total)
