@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_kv_cache import heads, values
+from test_gpu_kv_cache import SHAPES, heads, values
 
 pytestmark = pytest.mark.gpu
 
@@ -187,3 +187,33 @@ def test_a_large_value_that_later_rows_see(kv, dtype, H, Hkv, Tq):
     see = torch.arange(n, device="cuda") < (n - Tq + 1 + torch.arange(Tq, device="cuda")).view(1, Tq, 1)
     want = exact(q, values(k), values(v), 1 / math.sqrt(dh), see.expand(B, Tq, n))
     judge_rows(kv.attention(q, c, n, causal=True), want, BESIDE)
+
+
+# ------------------------------------------------------------------------------------------------ ordinary inputs
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("B,H,Hkv,dh,Tq,cap,lengths", SHAPES)
+def test_ordinary_inputs_in_norm(kv, B, H, Hkv, dh, Tq, cap, lengths, causal, dtype):
+    """A score is a sum over dh features of |q| (|z| + 15 s) ~ 5, codes' and zeros' parts apart, times scale: 5 sqrt(dh) ~ 50 at
+    most, with the parts' 2^-22 (bf16: the low codes' 2^-21) and some roundings, of which a random half cancels: rms 1e-6 of a
+    probability, and 2e-6 of the codes (check_mean_zero) at most: 3e-6 together in fp32, 1e-5 in bf16, whose scores take one part
+    and low codes.  (Probabilities of one part would be 2^-12 / sqrt(3) = 1.4e-4 off, a dropped last token of 20000 7e-3.)"""
+    c = kv.KVCache4(B, Hkv, dh, cap)
+    c.data.fill_(0xFF)
+    n = torch.tensor(lengths, device="cuda", dtype=torch.int32)
+    k, v = heads(B, Hkv, cap, dh, dtype, 11, 1.5), heads(B, Hkv, cap, dh, dtype, 12)
+    c.write(k, v, 0, n)
+    q = heads(B, H, Tq, dh, dtype, 13)
+    got = kv.attention(q, c, n, causal=causal)
+    kk, vv = values(k), values(v)
+    got_rows, want_rows = [], []
+    for b, m in enumerate(lengths):
+        for i in range(Tq):
+            see = max(0, m - Tq + 1 + i) if causal else m
+            if see == 0:
+                assert (got[b, :, i] == 0).all()
+                continue
+            at = slice(b, b + 1)
+            got_rows.append(got[at, :, i])
+            want_rows.append(exact(q[at, :, i:i + 1], kk[at, :, :see], vv[at, :, :see], 1 / math.sqrt(dh))[:, :, 0])
+    judge(torch.cat(got_rows), torch.cat(want_rows), 3e-6 if dtype == torch.float32 else 1e-5)
