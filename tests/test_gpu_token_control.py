@@ -327,3 +327,22 @@ def test_two_picks_at_once(tc):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(t, want[i]) for t in got[i])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,V,T,spread", [(260, 131071, 40, 50),        # the largest chunk of a row that a block takes, 16-bit marks
+                                          (130, 20000, 17000, 3)])      # and 32-bit ones
+def test_the_largest_chunks(tc, dtype, B, V, T, spread):
+    c = make(B, V, T, dtype, 31, spread=spread)
+    c["history"][:, ::9] = V - 1 - c["history"][:, ::9]                 # both ends of the row
+    args = (rules(tc, c), c["history"], c["lengths"], c["prompt"])
+    same_logits_of(tc.control_logits(c["logits"], *args), expect(c, False), T)
+    assert tc.pick_token(c["logits"], *args).tolist() == picks(expect(c, True))
+
+
+def same_logits_of(got, want, T):
+    """same_logits for penalties up to 2 T + 1: their roundings counted with that size."""
+    half = torch.finfo(got.dtype).eps / 2
+    got = got.double().cpu()
+    assert torch.equal(torch.isinf(got), torch.isinf(want)) and not torch.isnan(got).any()
+    assert ((got - want).abs() <= half * want.abs() + 6 * 2.0 ** -24 * (want.abs() + 4 * T + 80)).all()
