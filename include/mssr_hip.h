@@ -691,7 +691,7 @@ int mssr_kv4_attention(const mssr_kv4_attention_desc* desc, void* stream);
  * n-gram rule of onmt/translate/decode_strategy.py): penalties for tokens of the history, a bias, a grammar's mask, no
  * repeated n-gram; the arithmetic is stated in csrc/token_control.hip.  Writes the new logits (out), the pick (ids: the
  * largest, lowest index on ties, NaN above everything, `empty` where nothing is left), or both; out may be logits itself, and
- * overlaps it in no other way.
+ * overlaps it in no other way, nor the bias.  ids may lie in the history past its lengths.
  * Index arrays hold 32-bit integers, or 64-bit ones where their bit of index_bits is set.  Nothing in them is checked on the
  * host: history entries outside [0, V) are passed over, lengths are clamped to [0, T], a state below 0 leaves its row free,
  * one beyond the table allows nothing. */

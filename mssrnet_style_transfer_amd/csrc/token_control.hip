@@ -286,6 +286,12 @@ static bool tc_apart(const mssr_token_control_desc* d) {
     return gap >= row && gap <= d->ld * es - row;
 }
 
+// The new logits and the bias have no byte in common: a block reads its bias while others write.
+static bool tc_bias_apart(const mssr_token_control_desc* d) {
+    const int64_t es = d->dtype == MSSR_F32 ? 4 : 2, y = (int64_t)(intptr_t)d->out, z = (int64_t)(intptr_t)d->bias;
+    return y + ((d->B - 1) * d->ldo + d->V) * es <= z || z + ((d->B - 1) * d->bias_bs + d->V) * 4 <= y;
+}
+
 template <typename T>
 static void tc_launch(const TokenControlArgs& a, bool wide, unsigned grid, unsigned lds, hipStream_t st) {
     if (wide) token_control_kernel<T, uint32_t><<<grid, TC_THREADS, lds, st>>>(a);
@@ -321,6 +327,8 @@ extern "C" int mssr_token_control(const mssr_token_control_desc* d, void* stream
     const TcShape s = tc_shape(d->B, d->V, d->T, d->ids != nullptr);
     MSSR_REQUIRE(d->B <= TC_MAX_GRID / s.chunks, "token_control: %lld rows in one call", (long long)d->B);
     MSSR_REQUIRE(!d->out || tc_apart(d), "token_control: the new logits overlap the old ones without taking their place");
+    MSSR_REQUIRE(!d->bias || (d->bias_bs >= 0 && d->bias_bs <= TC_MAX_LD), "token_control: bias rows %lld apart", (long long)d->bias_bs);
+    MSSR_REQUIRE(!d->out || !d->bias || tc_bias_apart(d), "token_control: the new logits overlap the bias");
     MSSR_REQUIRE(!d->ids || s.chunks == 1 ||
                      (d->scratch && d->scratch_bytes >= d->B * s.chunks * (int64_t)sizeof(unsigned long long)),
                  "token_control: scratch of %lld bytes is too small", (long long)d->scratch_bytes);

@@ -177,7 +177,7 @@ def control_logits(logits, control=None, history=None, lengths=None, prompt_leng
     ``history``: int32 / int64 tensor [B, T] of tokens so far, any strides (a [T, B] buffer's transpose is read in place);
     entries outside the vocabulary are passed over.  ``lengths``: integer tensor [B], how many of them count (default: all).
     ``prompt_lengths``: integer tensor [B], frequency and presence count from there on.  ``out``: where to write; ``logits``
-    itself changes them in place (memory that overlaps theirs in another way is refused)."""
+    itself changes them in place (memory that overlaps theirs in another way, or the bias, is refused)."""
     who = "control_logits"
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
@@ -191,7 +191,7 @@ def control_logits(logits, control=None, history=None, lengths=None, prompt_leng
 def pick_token(logits, control=None, history=None, lengths=None, prompt_lengths=None, empty=-1, out=None):
     """The word with the largest controlled logit of every row, int64 [B] (or written to ``out``, an int32 / int64 tensor
     [B]): the lowest one on ties, NaN above everything as in torch.argmax, ``empty`` where every word is at minus infinity.
-    Other arguments as for ``control_logits``; the new logits are not written."""
+    Other arguments as for ``control_logits``; the new logits are not written.  ``out`` may lie in the history past ``lengths``."""
     who = "pick_token"
     if logits.dim() != 2:
         raise ValueError("%s: logits [B, V] expected (got %s)" % (who, tuple(logits.shape)))

@@ -243,3 +243,13 @@ def test_a_cached_search_that_fails_leaves_no_state():
     assert all(model.decoder.state[name] is None for name in ("src", "cache", "kv4_steps"))
     nothing = SimpleNamespace()                                         # a search of no steps asks nothing of the model
     assert greedy_decode_cached(nothing, cfg, mem, lens, 0).shape == (0, 3)
+
+
+def test_new_logits_over_the_bias_are_refused():
+    far = FAKE + (1 << 16)
+    for kw in (dict(out=far, bias=far), dict(out=far, bias=far + 4 * 99), dict(out=far, bias=far - 4 * 49),
+               dict(out=far, bias=far - 4 * 60, bias_bs=50), dict(out=far, bias=far, dtype=L.BF16, logits=FAKE)):
+        assert control(**kw) == 1, kw
+        assert b"overlap the bias" in L.load().mssr_last_error(), kw
+    for kw in (dict(out=far, bias=FAKE + 4096, bias_bs=-1), dict(out=far, bias=FAKE + 4096, bias_bs=1 << 40)):
+        assert control(**kw) == 1, kw
