@@ -307,12 +307,12 @@ __device__ __forceinline__ void kv4_finish(const Kv4AttnArgs& a, const Kv4Work& 
 //   scores   per group 4 products of 16 tokens; every quad of rows of the q operand holds the same rows, so lane
 //            (quad, n) finds token n of each product and keeps the one of its own 16 (one fp32 row: its parts are rows)
 //   p s      goes through LDS to become an operand: row 4 part + r, the parts add up at the end
-// Bound by memory where sentences are long or many: 16 sentences x 8 heads x 26000 tokens of 64 bf16 features (270 MB) 43 us
-// and 5 for the join, 58 us in a row of launches, 4.6 TB/s, the rate of a large copy; 512 x 8 heads x 65 .. 140 tokens 12.1 us,
-// 3 of them the launch (35 MB needed, 40 read: half blocks are the least).  By vector instructions and latency elsewhere: 8 x 8
-// heads with 4 fp32 rows each, 4000 .. 8190 tokens of 128 features (63 MB) 24 us and 4 for the join, 9 of which a sentence of
-// one block takes as well (some 1500 instructions before and after the loop; in it 420 vector and 56 matrix ones a block); one
-// sentence of 20 tokens 3.3 us.
+// Bound by memory where sentences are long or many: 16 sentences x 8 heads x 26000 tokens of 64 bf16 features (270 MB) 59 us in
+// a row of launches over as many caches, 5 of them the join, 4.6 TB/s, the rate of a large copy; 512 x 8 heads x 65 .. 140 tokens
+// 13.5 us, 3 of them the launch (35 MB needed, 40 read: half blocks are the least; 12.1 with one part of p s).  By vector
+// instructions and latency elsewhere: 8 x 8 heads with 4 fp32 rows each, 4000 .. 8190 tokens of 128 features (63 MB) 29 us, 4 of
+// them the join and 10 what a sentence of one block takes as well (some 1800 instructions before and after the loop and 500 for the first
+// units; in it 570 vector and 56 matrix ones a block); one sentence of 20 tokens 3.7 us.
 template <typename T, int NG, int R, int W>
 __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnArgs a) {
     constexpr bool F32 = sizeof(T) == 4;
@@ -566,9 +566,10 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnAr
 // score shared its error, and values about zero came out 2 % (2000 tokens) to 5 % (16000) off.  Scales and zeros are one a
 // token and reach the lanes through LDS; a group that is NaN has a NaN scale, its zero is taken as 0 so that rows that do not see
 // the token stay clean.
-// 24 x 4 heads with 20 rows each, 700 .. 2050 tokens of 96 bf16 features (17 MB): 18.9 us; 15.6 with one part of p s, 8 of
-// which a sentence of one block took as well (18.6 then with a second copy of the step for blocks without masks and with divisions: code that is run through
-// once is slow to fetch).
+// 24 x 4 heads with 20 rows each, 700 .. 2050 tokens of 96 bf16 features (17 MB): 20.2 us, 7.0 of which a sentence of one block
+// takes as well; 15.6 with one part of p s and one unit for all (18.6 then with a second copy of the step for blocks without
+// masks and with divisions: code that is run through once is slow to fetch).  104 .. 128 features spill registers (W = 8: 17 in
+// bf16 calls, 82 in fp32 ones): the same at 128 features 26 us, in fp32 42.
 template <typename T, int NG, int W>
 __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnArgs a) {
     constexpr bool F32 = sizeof(T) == 4;
@@ -730,10 +731,16 @@ __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_many_kernel(Kv4AttnA
                 for (int r = 0; r < 4; ++r) {
                     zs[g] = fmaf(s[t][r], z4[r], zs[g]);
                     y[t][r] = s[t][r] * v4[r];
-                    if (__builtin_expect(hidden, 0)) y[t][r] = 16 * t + 4 * quad + r < see ? y[t][r] : 0.f;
-                    most = fmaxf(most, y[t][r]);
                 }
             }
+            if (__builtin_expect(hidden, 0)) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[t][r] = 16 * t + 4 * quad + r < see ? y[t][r] : 0.f;
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) most = fmaxf(most, fmaxf(fmaxf(y[t][0], y[t][1]), fmaxf(y[t][2], y[t][3])));
             if (__any(__builtin_amdgcn_ldexpf(most, up[g]) > (float)(1 << KV4_FULL))) {
                 most = fmaxf(most, __shfl_xor(most, 16));
                 most = fmaxf(most, __shfl_xor(most, 32));
@@ -867,16 +874,17 @@ struct Kv4Shape { int rows, W, splits; int64_t units; };
 // How a call is cut: `longest` bounds the lengths (the capacity where the caller knows no better), nb is that in blocks of
 // 64 tokens, units the (sentence, key/value head, query rows) triples.  Measured on graph replays, us, "a x b" for a units of b
 // tokens, 64 bf16 features unless others are named:
-//   a wave each (W = 1) where units fill the chip: 2048 x 140 7.6 against 11.0 with four waves, 4096 x 1200 with 16 rows 83
-//     against 97, with 4 rows (96 fp32 features) 131 against 160; with one row 2048 x 1200 31 against 29
-//   eight waves where units are few: 64 x 1200 6.1 against 7.4, 512 x 1200 11.8 against 12.5; but 512 x 300 6.1 against 5.7,
-//     512 x 2500 of 128 fp32 features 44 against 42, many-row kernels on 512 units 10.9 against 8.0.  4 rows: 256 x 2500 15.1
-//     against 18.6, but 64 x 300 6.4 against 5.9
+//   a wave each (W = 1) where units fill the chip: 2048 x 140 9.3 against 12.1 with four waves, 4096 x 1200 with 16 rows 110
+//     against 127, with 4 rows 79 against 88 (96 fp32 features 134 - 142 against 137); with one row 2048 x 1200 38 against 38
+//   eight waves where units are few: 64 x 1200 6.1 against 7.4, 512 x 1200 11.9 against 11.8; but 512 x 300 6.9 against 6.6,
+//     512 x 2500 of 128 fp32 features 45 against 41, many-row kernels 512 x 1200 21.2 against 18.5 (256 x 1200 11.5 against 13.9).
+//     4 rows: 256 x 2500 16.2 against 18.3, but 64 x 300 7.8 against 7.3
 //   splits, whose joining costs a second launch (3 us), where a unit's waves would go round often and the chip has room: as
 //     many as give every CU a block, or two where two fit and there are several sentences (their lengths differ), and twice as
-//     many again for very long ones.  64 x 10000 15.3 against 25.4 unsplit (with 9 splits, blocks that do not fill the last
-//     round, 19.3), 128 fp32 features 24.7 against 46.1; 64 x 2500 9.0 against 8.2; 128 x 0 .. 32768 36 with 8 splits, 38
-//     with 4.  4 rows: 64 x 8190 17 against 27, of 128 fp32 features 32 against 61; 64 x 1000 9.6 against 8.5
+//     many again for very long ones.  64 x 10000 15.5 against 26.5 unsplit (with 9 splits, blocks that do not fill the last
+//     round, 18.2), 128 fp32 features 25 against 48; 64 x 2500 8.8 against 9.7 unsplit; 128 x 0 .. 32768 30.5 with 8 splits, 31.7
+//     with 4, 78 unsplit.  4 rows: 64 x 8190 17 against 30, of 128 fp32 features 28 against 55; 64 x 1000 9.8 against 9.2.  16
+//     rows: 64 x 2000 11.3 against 14.4, 64 x 1000 10.2 against 9.4
 static Kv4Shape kv4_shape(int64_t B, int Hkv, int NQ, int ng, int64_t longest) {
     Kv4Shape s;
     s.rows = NQ == 1 ? 1 : NQ <= 4 ? 4 : 16;
