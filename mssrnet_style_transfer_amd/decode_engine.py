@@ -773,8 +773,8 @@ def greedy_decode_ids(model, cfg, memory_bank, src_lengths, max_length, check_ev
     unspecified (tokens of the steps it kept running, then </s>); the caller cuts each sentence at its first </s>.
 
     ``control`` (token_control.TokenControl, no reference counterpart): rules for the logits of every step over the words
-    picked so far -- repetition penalties, biases, per-sentence grammar masks, no repeated n-grams.  A sentence whose
-    rules leave nothing ends (</s>)."""
+    picked so far -- repetition penalties, biases, per-sentence sets of allowed words, no repeated n-grams.  They are the
+    same at every step (a grammar's ``state`` does not move).  A sentence whose rules leave nothing ends (</s>)."""
     lib = L.load()
     params = decoder_params(model)
     dev = memory_bank.device

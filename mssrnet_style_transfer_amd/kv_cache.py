@@ -161,7 +161,7 @@ def attention(q, cache, lengths, scale=None, causal=False, longest=0):
     h // (H / heads).  ``lengths``: an int or an integer tensor [B].  ``scale``: 1 / sqrt(dim) if not given.  ``causal``: the
     rows are the sentence's last T tokens (their keys written already), row i sees the first lengths - T + 1 + i.  A row
     that sees no token gives zeros.  ``longest``: an upper bound of the lengths, if the caller knows one below the cache's
-    capacity (it shapes the launch, nothing else).  Returns [B, H, T, dim], a view of [B, T, H, dim] memory, in q's type;
+    capacity (it shapes the launch, nothing else).  Sums are fp32 ones of operands of 22 bits.  Returns [B, H, T, dim], a view of [B, T, H, dim] memory, in q's type;
     probabilities are not returned."""
     who = "kv_cache.attention"
     L.refuse_graph(who, q)
