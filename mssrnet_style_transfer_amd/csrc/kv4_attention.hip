@@ -16,8 +16,8 @@
 // values about zero one in three.  Powers of two keep the parts in fp16's range: a query row is scaled to a largest element in
 // [2^13, 2^14) (fp32: [2^9, 2^10); what is 2^-11 of it still has its 22 bits, the rest is off by at most 2^-34 of it).  Every
 // query row and group has its own for p s: the largest met so far lies in [2^6, 2^7) when the unit is chosen and may grow to
-// 2^15 before it is chosen anew (then the sums shrink); what is 2^-9 of it has its 22 bits, the rest is off by at most 2^-31 of it.
-// With one unit for the largest V scale of all rows, groups and tokens, an fp32 result was 3e-3 off where a value 1e6 times as
+// 2^15 before it is chosen anew (then the sums shrink); what is 2^-9 of it has its 22 bits, the rest is off by at most 2^-31 of
+// it.  With one unit for the largest V scale of all rows, groups and tokens, an fp32 result was 3e-3 off where a value 1e6 times as
 // large stood in a token that the row does not attend to.
 //
 // Where values are spread about zero, codes' and zeros' shares of the context nearly cancel, the more so the more tokens
@@ -27,8 +27,9 @@
 // in norm, and of bf16 ones 1 or 2 in 1000 are not the nearest number.
 //
 // A wave takes 64 tokens at a time; a row's running maximum moves only when a score passes it by more than 8, and units of
-// p s only as above (then that row's sums are rescaled), so that a block of tokens costs one comparison and no cross-lane reduction.  The W waves of a block
-// take every W-th 64 tokens of its share of the sentence and are joined through LDS; a second launch joins the shares.
+// p s only as above (then that row's sums are rescaled), so that a block of tokens costs one comparison and no cross-lane
+// reduction.  The W waves of a block take every W-th 64 tokens of its share of the sentence and are joined through LDS; a second
+// launch joins the shares.
 #include "kv4.hpp"
 
 namespace mssr {
@@ -65,7 +66,7 @@ struct Kv4AttnArgs {
 constexpr float KV4_LAZY = 8.f;          // log2 of how far a probability may pass 1 before a rescale
 constexpr int KV4_UP = 7;                // log2 of what the largest p s is held below when its unit is chosen,
 constexpr int KV4_FULL = 15;             // and what it may grow to before the unit is chosen anew
-constexpr int KV4_MOST_UP = 40;          // what no p s is held more than 2^this times: smaller ones are nothing beside the row's sums
+constexpr int KV4_MOST_UP = 40;          // no p s is held more than 2^this times: smaller ones are nothing beside the row's sums
 constexpr float KV4_NONE = -3e38f;       // the reference of a row that has seen no token: 2^(-inf - KV4_NONE) is 0
 constexpr float KV4_MID = 7.5f;          // what is taken from codes and added, times the scale, to zeros
 constexpr int KV4_PS_PARTS = 2;          // fp16 parts of p s
@@ -311,8 +312,8 @@ __device__ __forceinline__ void kv4_finish(const Kv4AttnArgs& a, const Kv4Work& 
 // a row of launches over as many caches, 5 of them the join, 4.6 TB/s, the rate of a large copy; 512 x 8 heads x 65 .. 140 tokens
 // 13.5 us, 3 of them the launch (35 MB needed, 40 read: half blocks are the least; 12.1 with one part of p s).  By vector
 // instructions and latency elsewhere: 8 x 8 heads with 4 fp32 rows each, 4000 .. 8190 tokens of 128 features (63 MB) 29 us, 4 of
-// them the join and 10 what a sentence of one block takes as well (some 1800 instructions before and after the loop and 500 for the first
-// units; in it 570 vector and 56 matrix ones a block); one sentence of 20 tokens 3.7 us.
+// them the join and 10 what a sentence of one block takes as well (some 1800 instructions before and after the loop and 500 for
+// the first units; in it 570 vector and 56 matrix ones a block); one sentence of 20 tokens 3.7 us.
 template <typename T, int NG, int R, int W>
 __global__ __launch_bounds__(64 * kv4_waves(W), 2) void kv4_few_kernel(Kv4AttnArgs a) {
     constexpr bool F32 = sizeof(T) == 4;
